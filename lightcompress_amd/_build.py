@@ -21,8 +21,12 @@ LIB = LIB_DIR / 'liblcq.so'
 
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 ARCH = 'gfx950'
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 -- some of their forms have given wrong results
+# on MI355X, and -O3 makes them from ordinary float code by itself (the host pass does not know
+# the feature and warns, harmlessly)
 CFLAGS = ['-O3', '-fPIC', '-std=c++17', f'--offload-arch={ARCH}', '-Wall',
           '-Wno-unused-function', '-Wno-unused-variable', '-ffp-contract=off',
+          '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
           f'-I{INCLUDE}', f'-I{CSRC}']
 
 
@@ -50,7 +54,7 @@ def build(verbose: bool = False, defines=(), lib: Path = LIB, build_dir: Path = 
     build_dir.mkdir(parents=True, exist_ok=True)
     lib.parent.mkdir(parents=True, exist_ok=True)
     sources = sorted(CSRC.glob('*.hip'))
-    headers = sorted(CSRC.glob('*.h')) + sorted(INCLUDE.glob('*.h'))
+    headers = sorted(CSRC.glob('*.h')) + sorted(INCLUDE.glob('*.h')) + [Path(__file__)]
     jobs = min(len(sources), int(os.environ.get('MAX_JOBS', '8')))
     with cf.ThreadPoolExecutor(max_workers=max(jobs, 1)) as ex:
         objs = list(ex.map(lambda s: _compile(s, headers, build_dir, defines), sources))

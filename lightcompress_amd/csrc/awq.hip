@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(64) k_sqdiff_p2(const double* part, int nparts
 // The reference materialises the DT broadcast product, so every product is rounded to DT
 // before the fp32 sum: that rules out MFMA (exact products). VALU design: the candidate
 // weights live unpacked in VGPRs, x tiles are fp32 in LDS and read as wave-uniform broadcasts,
-// products go through v_pk_mul_f32 + v_cvt_pk_bf16_f32 (RNE) and v_pk_add_f32 into 8 partial
+// products go through v_mul_f32 + v_cvt_pk_bf16_f32 (RNE) and v_add_f32 into 8 partial
 // sums (k mod 8) reduced by a halving tree (torch-CPU's vectorised order), the per-step
 // squared-error sums and the original outputs sit in LDS so the token loop stays rolled.
 // ----------------------------------------------------------------------------------------
@@ -387,8 +387,8 @@ __device__ __forceinline__ float xor1(float v) {  // value of the partner lane (
 template <int DT, int G, int R>
 __device__ __forceinline__ void dot_rows(const float* __restrict__ xr,
                                          const float (&q)[R][G / 2], int h, float (&out)[R]) {
-  // packed fp32 products and sums (v_pk_mul_f32 / v_pk_add_f32): measured 1.26x faster than
-  // the same work as scalar v_mul_f32 / v_add_f32 (49 % more instructions)
+  // pairs written as 2-vectors; the build has no packed fp32 instructions, so each is two
+  // scalar ones (as packed ones this loop took 24.9 instead of 30.7 ms at 14336 x 4096)
   v2f a0[R], a1[R];
 #pragma unroll
   for (int j = 0; j < R; ++j) a0[j] = a1[j] = v2f{0.f, 0.f};
@@ -468,7 +468,7 @@ struct ClipTile {
 template <int DT>
 __device__ __forceinline__ uint16_t dt_bits(float v) {  // v is a DT value
   if constexpr (DT == LCQ_BF16) return (uint16_t)(__float_as_uint(v) >> 16);
-  else return __builtin_bit_cast(uint16_t, (_Float16)v);
+  else return __builtin_bit_cast(uint16_t, to_f16(v));
 }
 template <int DT>
 __device__ __forceinline__ float dt_val(uint16_t b) {
@@ -676,8 +676,8 @@ __global__ void __launch_bounds__(2 * CROWS, G >= 256 ? 1 : 2)
 // (profiles/r3b_clip_pmc.json). Here a lane is a token and keeps that token's 128 x values
 // of the group in VGPRs for all of a wave's rows; the candidate weights of every (row, step)
 // are precomputed once (k_clip_qtable, the same arithmetic) and read as wave-uniform scalar
-// loads, so the inner loop is VALU only: per product pair one v_pk_mul_f32, two
-// v_cvt_pk_bf16_f32 and one v_pk_add_f32, in the same 8 partial sums and halving tree as
+// loads, so the inner loop is VALU only: per product pair two v_mul_f32, two
+// v_cvt_pk_bf16_f32 and two v_add_f32, in the same 8 partial sums and halving tree as
 // dot_rows. A wave walks ALL tokens of its rows in order (64 per chunk), so each step's
 // squared-error sum is accumulated in token order exactly as in k_auto_clip: the per-token
 // errors of three rows go through a small per-wave LDS transpose and one lane per
@@ -1025,8 +1025,8 @@ __global__ void __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(3)))   
 //  * a set's candidate rows ([TW_R][11][128] fp32, the k_clip_qtable table) come into one of
 //    two LDS buffers by LDS-DMA, issued one set ahead (no VGPRs, no wait inside the compute);
 //  * the compute reads them as wave-uniform ds_read_b128 broadcasts (4 per 16 products, the
-//    next 16 in flight under the current 16's 32 VALU): per product pair one v_pk_mul_f32,
-//    two v_cvt_pk_bf16_f32, one v_pk_add_f32, the 8 partial sums and halving tree of dot_rows;
+//    next 16 in flight under the current 16's VALU): per product pair two v_mul_f32,
+//    two v_cvt_pk_bf16_f32, two v_add_f32, the 8 partial sums and halving tree of dot_rows;
 //  * each (row, step)'s per-token errors (DT bits) go to an LDS row [pair][token]; one set
 //    later one wave (rotating) sums each pair's T errors sequentially in token order -- the
 //    order k_auto_clip and k_auto_clip_tl use -- and picks the first strict minimum.

@@ -86,7 +86,15 @@ __device__ __forceinline__ float div_exact(float a, float b, float rb) {
              ? q
              : __fdiv_rn(a, b);
 }
-__device__ __forceinline__ float f16_rne(float f) { return (float)(_Float16)f; }
+// fp32 -> fp16 of a value that is itself a rounded fp32 result. The empty asm keeps the producing
+// operation apart: without it the compiler folds a product (or fma) and the conversion into one
+// v_fma_mixlo_f16, which rounds once where the reference's torch op rounds twice (to fp32, then
+// to fp16) -- x * s of an fp16 tensor then differs in its last bit at double-rounding ties.
+__device__ __forceinline__ _Float16 to_f16(float f) {
+  asm("" : "+v"(f));
+  return (_Float16)f;
+}
+__device__ __forceinline__ float f16_rne(float f) { return (float)to_f16(f); }
 
 // Translation units that define LCQ_BF16_HW before including this header (the streaming
 // quant kernels) round on the conversion instruction everywhere (rnd, st8); the rest keep
@@ -176,7 +184,7 @@ __device__ __forceinline__ void st1(void* p, int64_t i, float v) {
   if constexpr (DT == LCQ_F32) reinterpret_cast<float*>(p)[i] = v;
   else if constexpr (DT == LCQ_BF16)
     reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(__float_as_uint(LCQ_BF16_ROUND(v)) >> 16);
-  else if constexpr (DT == LCQ_F16) reinterpret_cast<_Float16*>(p)[i] = (_Float16)v;
+  else if constexpr (DT == LCQ_F16) reinterpret_cast<_Float16*>(p)[i] = to_f16(v);
 }
 
 // 8 consecutive elements <-> float[8] with 16-byte vector accesses (Guideline 13)
@@ -209,8 +217,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return (__float_as_uint(LCQ_BF16_ROUND(a)) >> 16) |
            (__float_as_uint(LCQ_BF16_ROUND(b)) & 0xffff0000u);
   } else {
-    uint16_t lo = __builtin_bit_cast(uint16_t, (_Float16)a);
-    uint16_t hi = __builtin_bit_cast(uint16_t, (_Float16)b);
+    uint16_t lo = __builtin_bit_cast(uint16_t, to_f16(a));
+    uint16_t hi = __builtin_bit_cast(uint16_t, to_f16(b));
     return (uint32_t)lo | ((uint32_t)hi << 16);
   }
 }
