@@ -712,6 +712,38 @@ int lcq_gemm_sq_diff(const void* a, int dtype, int64_t lda, int64_t m, int64_t k
                      int64_t ldr, void* workspace, int64_t ws_bytes, void* out_f32, int slot,
                      void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Products with 4-bit packed weights and group scales: the forward of the deployed linears, on
+ * the buffers the deploy path stores (the reference's VllmRealQuantLinear /
+ * AutoawqRealQuantLinear.forward raise; module_utils.py:855-1158 define the layouts).
+ *   y[m, n] = sum_k x[m, k] (c[n, k] - z[n, k / group]) s[n, k / group] (+ bias[n])
+ * layout 0 (vLLM, lcq_pack_vllm of 4-bit symmetric codes): qweight int32 [n, k/8], nibble i of a
+ *   word = code of column 8 j + i, z = 8; scales fp16 [n, k/group]; qzeros NULL.
+ * layout 1 (AutoAWQ, lcq_pack_autoawq_gemm): qweight int32 [k, n/8] and qzeros int32
+ *   [k/group, n/8], nibble i = column 8 j + {0,2,4,6,1,3,5,7}[i]; scales fp16 [k/group, n].
+ * x [m, k] bf16 / fp16 (row stride ldx, a multiple of 8; 16-byte aligned), bias [n] and y [m, n]
+ * (row stride ldy) in the same dtype. group % 32 == 0, k % group == 0, layout 1: n % 8 == 0; any
+ * m >= 0 (0: nothing to do). Codes and zero points enter exactly, sums are fp32 (a fixed order:
+ * the same call gives the same bits), one rounding at the end. A row of x with an infinity or a
+ * NaN gives NaN in that row.
+ * ------------------------------------------------------------------------------------- */
+int lcq_int4_gemm(const void* x, int dtype, int64_t ldx, int64_t m, int64_t k,
+                  const void* qweight, const void* scales, const void* qzeros, int layout,
+                  int64_t group, int64_t n, const void* bias, void* y, int64_t ldy, void* stream);
+
+/* lcq_int4_gemm for the G routed experts of an MoE projection in one launch (the expert loop of
+ * the reference's models/deepseekv3.py MoE forward on packed experts). Rows and groups as in
+ * lcq_fp8_gemm_grouped: group g owns rows [row_off[g], row_off[g + 1]) (row_off: DEVICE int64
+ * [G + 1], ascending; clamped to [0, rows]); rows outside every group are left as they were.
+ * With a_rows (DEVICE int64 [rows]) row i reads x row a_rows[i] (out of [0, x_rows): zeros), else
+ * x row i. wtab: DEVICE int64 [nsets][G][3] = qweight, scales, qzeros addresses (qzeros ignored in
+ * layout 0), each [n, k] matrix as above. nsets 2: y [2][rows][n]; with silu_mul set 0 = gate,
+ * set 1 = up and y [rows][n] = rnd(silu(gate) * up), the two products kept in fp32. */
+int lcq_int4_gemm_grouped(const void* x, int dtype, int64_t ldx, int64_t x_rows,
+                          const int64_t* a_rows, int64_t rows, const int64_t* row_off,
+                          const int64_t* wtab, int64_t G, int nsets, int silu_mul, int layout,
+                          int64_t group, int64_t n, int64_t k, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

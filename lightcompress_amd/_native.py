@@ -6,6 +6,7 @@ ROCm device, the call raises. This is the binding a maintainer adds to the refer
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import re
@@ -143,6 +144,10 @@ SIGNATURES = {
     'lcq_gemm_sq_diff_workspace_bytes': ([_i64, _i64], _i64),
     'lcq_gemm_sq_diff': ([_vp, _int, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp,
                           _i64, _vp, _int, _vp], _int),
+    'lcq_int4_gemm': ([_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _int, _i64, _i64, _vp, _vp,
+                       _i64, _vp], _int),
+    'lcq_int4_gemm_grouped': ([_vp, _int, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _int, _int,
+                               _int, _i64, _i64, _i64, _vp, _vp], _int),
     'lcq_fp_emul_quant': ([_vp, _int, _i64, _i64, _i64, _int, _int, _vp, _int, _vp], _int),
 }
 
@@ -208,6 +213,14 @@ def ptr_strided(t):
 
 def stream_of(t: torch.Tensor):
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def on_device(t: torch.Tensor):
+    """Context in which t's device is the current one (a launch on another device's stream is an
+    error); does nothing where it already is."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 class KernelTimer:

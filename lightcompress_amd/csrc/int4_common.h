@@ -1,0 +1,61 @@
+// Fragments of the 4-bit weight kernels (int4.hip): packed words -> MFMA operands.
+//
+// A code c (0..15) becomes the float 16 + c by placing its four bits at the top of the mantissa of
+// 16.0 (bf16 0x4180 | c << 3, fp16 0x4c00 | c << 6): exact, one shift and one and-or for two
+// codes. With u = 16 + c the product with the weight (c - z) s of one group is
+//   s * ( sum_k x_k u_k  -  (16 + z) sum_k x_k ),
+// so a group costs its MFMAs, the sum of its x (one more MFMA against ones, shared by all the
+// columns of a wave) and one fp32 multiply-add per output. The codes stay exact; the offset of
+// 16 costs at most 2 more bits of the fp32 sum than a signed code would.
+#pragma once
+
+#include "lcq_common.h"
+
+namespace lcq {
+
+typedef short i4_v8s __attribute__((ext_vector_type(8)));
+typedef __bf16 i4_v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 i4_v8h __attribute__((ext_vector_type(8)));
+typedef float i4_v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t i4_v4u __attribute__((ext_vector_type(4)));
+
+template <int DT>
+__device__ __forceinline__ i4_v4f i4_mfma(i4_v4u a, i4_v4u b, i4_v4f c) {
+  if constexpr (DT == LCQ_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(i4_v8bf, a),
+                                                   __builtin_bit_cast(i4_v8bf, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(i4_v8h, a),
+                                                  __builtin_bit_cast(i4_v8h, b), c, 0, 0, 0);
+}
+
+// 1.0 in both halves
+template <int DT>
+constexpr uint32_t i4_ones = DT == LCQ_BF16 ? 0x3f803f80u : 0x3c003c00u;
+
+// nibbles P and P + 4 of w as 16 + code in the low and high half (P = 0..3)
+template <int DT, int P>
+__device__ __forceinline__ uint32_t i4_pair(uint32_t w) {
+  constexpr int at = DT == LCQ_BF16 ? 3 : 6;  // target bit of the code
+  constexpr uint32_t mask = DT == LCQ_BF16 ? 0x00780078u : 0x03c003c0u;
+  constexpr uint32_t base = DT == LCQ_BF16 ? 0x41804180u : 0x4c004c00u;
+  constexpr int sh = at - 4 * P;
+  if constexpr (sh >= 0) return ((w << sh) & mask) | base;
+  else return ((w >> -sh) & mask) | base;
+}
+
+// one word of 8 codes along k as a B fragment, elements in the order 0 4 1 5 2 6 3 7
+template <int DT>
+__device__ __forceinline__ i4_v4u i4_word(uint32_t w) {
+  return i4_v4u{i4_pair<DT, 0>(w), i4_pair<DT, 1>(w), i4_pair<DT, 2>(w), i4_pair<DT, 3>(w)};
+}
+
+// 8 consecutive x values as an A fragment in that order
+__device__ __forceinline__ i4_v4u i4_xorder(i4_v4u d) {
+  return i4_v4u{__builtin_amdgcn_perm(d.z, d.x, 0x05040100u),
+                __builtin_amdgcn_perm(d.z, d.x, 0x07060302u),
+                __builtin_amdgcn_perm(d.w, d.y, 0x05040100u),
+                __builtin_amdgcn_perm(d.w, d.y, 0x07060302u)};
+}
+
+}  // namespace lcq

@@ -1405,3 +1405,142 @@ def hqq_proximal(w2: torch.Tensor, group: int, scales: torch.Tensor, zeros: torc
            int(qmax), float(lp_norm), float(beta), int(iters), N.ptr(ws), ws.numel(),
            N.ptr(state), N.stream_of(w2))
     return s, z, state
+
+
+# ---------------------------------------------------------------------------------------
+# products with 4-bit packed weights (the deployed linears' forward)
+# ---------------------------------------------------------------------------------------
+INT4_LAYOUTS = {'vllm': 0, 'autoawq': 1}
+
+
+def _same_device(ref: torch.Tensor, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != ref.device:
+            raise ValueError(f'{name} is on {t.device}, not on {ref.device}')
+
+
+def _int4_weight(qweight, scales, qzeros):
+    """(layout, n, k, group) of a packed weight after checking its tensors."""
+    layout = 'vllm' if qzeros is None else 'autoawq'
+    if qweight.dtype != torch.int32 or qweight.dim() != 2 or not qweight.is_contiguous():
+        raise TypeError('qweight must be a contiguous 2-D int32 tensor')
+    if scales.dtype != torch.float16 or scales.dim() != 2 or not scales.is_contiguous():
+        raise TypeError('scales must be a contiguous 2-D fp16 tensor')
+    if layout == 'vllm':
+        n, k = qweight.shape[0], qweight.shape[1] * 8
+        ng, ns = scales.shape[1], scales.shape[0]
+    else:
+        k, n = qweight.shape[0], qweight.shape[1] * 8
+        ng, ns = scales.shape
+        if (qzeros.dtype != torch.int32 or not qzeros.is_contiguous()
+                or tuple(qzeros.shape) != (ng, n // 8)):
+            raise ValueError(f'qzeros must be contiguous int32 [{ng}, {n // 8}]')
+        _same_device(qweight, qzeros=qzeros)
+    if n == 0 or k == 0 or ns != n or ng == 0 or k % ng:
+        raise ValueError(f'scales {tuple(scales.shape)} do not fit a {layout} weight [{n}, {k}]')
+    if (k // ng) % 32:
+        raise ValueError(f'group size {k // ng} is not a multiple of 32')
+    _same_device(qweight, scales=scales)
+    if qweight.data_ptr() % 16 or scales.data_ptr() % 16:
+        raise ValueError('packed weights and scales must be 16-byte aligned')
+    return layout, n, k, k // ng
+
+
+def _int4_x(x: torch.Tensor, k: int) -> torch.Tensor:
+    """x as rows the kernels can read: 2-D, rows 16-byte aligned, columns contiguous."""
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f'bf16 / fp16 activations only, got {x.dtype}')
+    if x.dim() == 0 or x.shape[-1] != k:
+        raise ValueError(f'x has {x.shape[-1] if x.dim() else 0} columns, the weight {k}')
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.stride(0) < k or x2.data_ptr() % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    return x2
+
+
+def int4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
+                qzeros: torch.Tensor | None = None, bias: torch.Tensor | None = None
+                ) -> torch.Tensor:
+    """x [..., k] (bf16 / fp16) times a 4-bit packed weight with group scales, plus bias [n].
+
+    Without qzeros: the vLLM layout (qweight int32 [n, k/8] from ``pack_vllm`` of symmetric 4-bit
+    codes, scales fp16 [n, k/group]). With qzeros: the AutoAWQ layout of ``pack_autoawq_gemm``
+    (qweight [k, n/8], scales [k/group, n], qzeros [k/group, n/8]). The group size follows from
+    the shapes (a multiple of 32). Codes enter exactly, sums are fp32, the result is rounded once
+    to x's dtype. Not differentiable."""
+    layout, n, k, group = _int4_weight(qweight, scales, qzeros)
+    x2 = _int4_x(x, k)
+    _same_device(x2, qweight=qweight, bias=bias)
+    if bias is not None and (bias.dtype != x.dtype or bias.dim() != 1 or bias.numel() != n
+                             or not bias.is_contiguous()):
+        raise ValueError(f'bias must be a contiguous [{n}] tensor in the dtype of x')
+    y = torch.empty((x2.shape[0], n), dtype=x.dtype, device=x2.device)
+    with N.on_device(x2):
+        N.call('lcq_int4_gemm', N.ptr_strided(x2), N.dt(x2), x2.stride(0), x2.shape[0], k,
+               N.ptr(qweight), N.ptr(scales), N.ptr(qzeros), INT4_LAYOUTS[layout], group, n,
+               N.ptr(bias), N.ptr(y), n, N.stream_of(x2))
+    N.note_work('lcq_int4_gemm', 2.0 * x2.shape[0] * n * k)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
+
+
+def int4_weight_table(weights, device) -> torch.Tensor:
+    """Device table [G, 3] int64 of (qweight, scales, qzeros) addresses for int4_linear_grouped,
+    after checking every entry: tuples (qweight, scales) or (qweight, scales, None) in the vLLM
+    layout, (qweight, scales, qzeros) in the AutoAWQ one, all of one layout, shape and group. The
+    tensors must outlive every launch that reads the table (the caller keeps them with it)."""
+    rows, shape = [], None
+    device = torch.device(device)
+    for w in weights:
+        qw, s, z = w if len(w) == 3 else (*w, None)
+        got = _int4_weight(qw, s, z)
+        if shape is None:
+            shape = got
+        if got != shape:
+            raise ValueError(f'grouped int4 weights differ: {got} vs {shape}')
+        if qw.device.type != device.type or (device.index is not None and qw.device != device):
+            raise ValueError(f'grouped int4 weights on {qw.device}, table on {device}')
+        rows.append((qw.data_ptr(), s.data_ptr(), z.data_ptr() if z is not None else 0))
+    if not rows:
+        raise ValueError('no weights')
+    return torch.tensor(rows, dtype=torch.int64).to(device)
+
+
+def int4_linear_grouped(x: torch.Tensor, row_off: torch.Tensor, wtab: torch.Tensor, n: int,
+                        group: int, layout: str = 'vllm', a_rows: torch.Tensor | None = None,
+                        silu_mul: bool = False) -> torch.Tensor:
+    """One launch of G products with 4-bit packed weights (the routed experts of an MoE
+    projection), for one or two weight sets. Rows: the token slots sorted by group, row_off int64
+    [G + 1] on the device (group g = rows [row_off[g], row_off[g + 1])). With ``a_rows`` (int64
+    [rows] on the device) sorted row i is x[a_rows[i]] -- the gather happens in the kernel -- else
+    x itself is sorted. wtab from int4_weight_table, [G, 3] or [2, G, 3] (two sets: gate and up of
+    the same rows), all [n, k] with this group size and layout. Returns y [rows, n], or
+    [2, rows, n] for two sets; ``silu_mul`` (two sets = gate, up): h [rows, n] = silu(gate) * up,
+    formed in fp32 and rounded once. Rows outside every group are not written."""
+    if layout not in INT4_LAYOUTS:
+        raise ValueError(f'layout must be one of {sorted(INT4_LAYOUTS)}')
+    if x.dim() != 2:
+        raise ValueError('x must be 2-D')
+    k = x.shape[1]
+    x2 = _int4_x(x, k)
+    nsets = 1 if wtab.dim() == 2 else wtab.shape[0]
+    if (wtab.dtype != torch.int64 or wtab.dim() not in (2, 3) or wtab.shape[-1] != 3
+            or nsets not in (1, 2) or not wtab.is_contiguous()):
+        raise ValueError('wtab must be contiguous int64 [G, 3] or [2, G, 3]')
+    G = wtab.shape[-2]
+    if row_off.dtype != torch.int64 or row_off.numel() != G + 1 or not row_off.is_contiguous():
+        raise ValueError('row_off must be contiguous int64 [G + 1]')
+    if a_rows is not None and (a_rows.dtype != torch.int64 or a_rows.dim() != 1
+                               or not a_rows.is_contiguous()):
+        raise ValueError('a_rows must be a contiguous int64 vector')
+    if silu_mul and nsets != 2:
+        raise ValueError('silu_mul takes the gate and up tables ([2, G, 3])')
+    _same_device(x2, row_off=row_off, wtab=wtab, a_rows=a_rows)
+    rows = x2.shape[0] if a_rows is None else a_rows.numel()
+    y = torch.empty((rows, n) if nsets == 1 or silu_mul else (nsets, rows, n), dtype=x.dtype,
+                    device=x2.device)
+    with N.on_device(x2):
+        N.call('lcq_int4_gemm_grouped', N.ptr_strided(x2), N.dt(x2), x2.stride(0), x2.shape[0],
+               N.ptr(a_rows), rows, N.ptr(row_off), N.ptr(wtab), G, nsets, int(bool(silu_mul)),
+               INT4_LAYOUTS[layout], int(group), int(n), k, N.ptr(y), N.stream_of(x2))
+    N.note_work('lcq_int4_gemm_grouped', 2.0 * rows * n * k * nsets)
+    return y

@@ -1,0 +1,185 @@
+"""Products with 4-bit packed weights (lcq_int4_gemm, lcq_int4_gemm_grouped) against the 64-bit
+oracle: both deploy layouts, group sizes, row counts from one up, ragged groups, strides."""
+import pytest
+import torch
+
+from oracle import int4_ref as R
+
+pytestmark = pytest.mark.gpu
+
+LAYOUTS = ['vllm', 'autoawq']
+DTYPES = [torch.bfloat16, torch.float16]
+
+
+def weight(g, layout, n, k, group, dev):
+    """Random words (every code occurs), fp16 scales, zero points 0..15 in the AutoAWQ layout."""
+    ng = k // group
+
+    def words(*shape):
+        return torch.randint(-2**31, 2**31, shape, generator=g, dtype=torch.int64).to(
+            torch.int32).to(dev)
+
+    def sc(*shape):
+        return (torch.rand(*shape, generator=g) * 0.02 + 0.002).to(torch.float16).to(dev)
+    if layout == 'vllm':
+        return words(n, k // 8), sc(n, ng), None
+    return words(k, n // 8), sc(ng, n), words(ng, n // 8)
+
+
+def acts(g, *shape, dt, dev):
+    x = torch.randn(*shape, generator=g)
+    x[..., :: 37] *= 12          # outlier channels
+    return x.to(dt).to(dev)
+
+
+@pytest.mark.parametrize('layout', LAYOUTS)
+@pytest.mark.parametrize('dt', DTYPES)
+@pytest.mark.parametrize('m,n,k,group', [
+    (1, 256, 512, 128), (1, 8, 32, 32), (2, 40, 96, 96), (3, 72, 320, 32), (5, 264, 384, 64),
+    (16, 128, 1024, 128), (17, 136, 1024, 1024), (31, 520, 4096, 128), (33, 64, 1056, 1056),
+    (48, 1024, 256, 256), (64, 256, 640, 64), (65, 392, 2048, 128), (129, 640, 1152, 128),
+    (200, 328, 512, 32), (257, 512, 768, 128), (511, 200, 512, 512), (1, 4096, 4096, 128),
+    (4, 2048, 7168, 128), (300, 1288, 2048, 64)])
+def test_linear(dev, layout, dt, m, n, k, group):
+    from lightcompress_amd import ops
+    g = torch.Generator().manual_seed(m * 7919 + n * 31 + k + group)
+    w = weight(g, layout, n, k, group, dev)
+    x = acts(g, m, k, dt=dt, dev=dev)
+    got = ops.int4_linear(x, *w)
+    assert got.shape == (m, n) and got.dtype == dt
+    y, tol = R.linear(x, *w)
+    assert R.close(got, y, tol)
+    assert torch.equal(got, ops.int4_linear(x, *w))       # the same call, the same bits
+
+
+@pytest.mark.parametrize('m', [1, 16, 70, 300])
+def test_linear_odd_columns_vllm(dev, m):
+    """n of the vLLM layout is any number."""
+    from lightcompress_amd import ops
+    g = torch.Generator().manual_seed(m)
+    for n in (1, 15, 33, 131, 257):
+        w = weight(g, 'vllm', n, 256, 64, dev)
+        x = acts(g, m, 256, dt=torch.bfloat16, dev=dev)
+        y, tol = R.linear(x, *w)
+        assert R.close(ops.int4_linear(x, *w), y, tol), n
+
+
+@pytest.mark.parametrize('layout', LAYOUTS)
+@pytest.mark.parametrize('m', [3, 150])
+def test_linear_shapes_strides_bias(dev, layout, m):
+    from lightcompress_amd import ops
+    g = torch.Generator().manual_seed(5)
+    n, k = 264, 512
+    w = weight(g, layout, n, k, 128, dev)
+    b = torch.randn(n, generator=g).to(torch.bfloat16).to(dev)
+    big = acts(g, m, 2, k + 24, dt=torch.bfloat16, dev=dev)
+    for x in (big[..., 8:k + 8],          # 3-D, row stride k + 24
+              big[..., 3:k + 3],          # rows not 16-byte aligned
+              big[:, 0, :k], big[:, 1, :k].unsqueeze(1),
+              big[..., :k].transpose(0, 1)):
+        got = ops.int4_linear(x, *w, bias=b)
+        assert got.shape == (*x.shape[:-1], n)
+        y, tol = R.linear(x.reshape(-1, k), *w, bias=b)
+        assert R.close(got.reshape(-1, n), y, tol)
+    assert ops.int4_linear(big[:0, 0, :k], *w).shape == (0, n)
+
+
+@pytest.mark.parametrize('layout', LAYOUTS)
+@pytest.mark.parametrize('m', [4, 140])
+def test_linear_nan_and_inf_stay_in_their_row(dev, layout, m):
+    from lightcompress_amd import ops
+    g = torch.Generator().manual_seed(8)
+    w = weight(g, layout, 256, 512, 64, dev)
+    x = acts(g, m, 512, dt=torch.float16, dev=dev)
+    x[1, 100], x[3, 511] = float('nan'), float('inf')
+    got = ops.int4_linear(x, *w)
+    assert got[[1, 3]].isnan().all()
+    keep = [i for i in range(m) if i not in (1, 3)]
+    y, tol = R.linear(x[keep], *w)
+    assert R.close(got[keep], y, tol)
+
+
+@pytest.mark.parametrize('layout', LAYOUTS)
+@pytest.mark.parametrize('dt', DTYPES)
+@pytest.mark.parametrize('counts,n,k,group', [
+    ([1], 128, 256, 128), ([0, 3, 0, 1, 0], 264, 512, 32), ([16, 17, 15, 0, 64], 136, 384, 128),
+    ([0] * 70 + [5] + [0] * 90 + [33, 1], 128, 256, 64), ([300, 1, 129, 0, 40], 520, 1024, 128),
+    ([2] * 40, 72, 160, 160)])
+def test_grouped(dev, layout, dt, counts, n, k, group):
+    """One and two weight sets, the SiLU product, gathered and sorted rows."""
+    from lightcompress_amd import ops
+    g = torch.Generator().manual_seed(sum(counts) + n)
+    rows, E = sum(counts), len(counts)
+    off = torch.tensor([0] + counts).cumsum(0)
+    ws = [[weight(g, layout, n, k, group, dev) for _ in range(E)] for _ in range(2)]
+    tabs = [ops.int4_weight_table(w, dev) for w in ws]
+    both = torch.stack(tabs).contiguous()
+    x = acts(g, rows, k, dt=dt, dev=dev)
+    pick = torch.randint(0, rows, (rows,), generator=g)
+    for src in (None, pick):
+        xs = x if src is None else x[src.to(dev)]
+        kw = dict(layout=layout, a_rows=None if src is None else src.to(dev))
+        one = ops.int4_linear_grouped(x, off.to(dev), tabs[0], n, group, **kw)
+        two = ops.int4_linear_grouped(x, off.to(dev), both, n, group, **kw)
+        h = ops.int4_linear_grouped(x, off.to(dev), both, n, group, silu_mul=True, **kw)
+        assert one.shape == (rows, n) and two.shape == (2, rows, n) and h.shape == (rows, n)
+        for e in range(E):
+            s = slice(int(off[e]), int(off[e + 1]))
+            if s.start == s.stop:
+                continue
+            gu = [R.linear(xs[s], *w[e]) for w in ws]
+            assert R.close(one[s], *gu[0])
+            assert R.close(two[0, s], *gu[0]) and R.close(two[1, s], *gu[1])
+            assert R.close(h[s], *R.silu_mul(*gu))
+
+
+def test_grouped_rows_outside_groups_and_bad_gather(dev):
+    """Rows behind the last group stay as they were; a gather index out of range reads zeros;
+    offsets outside the rows are clamped."""
+    from lightcompress_amd import _native as N
+    from lightcompress_amd import ops
+    g = torch.Generator().manual_seed(3)
+    n, k, rows = 128, 256, 40
+    ws = [weight(g, 'vllm', n, k, 128, dev) for _ in range(3)]
+    tab = ops.int4_weight_table(ws, dev)
+    x = acts(g, rows, k, dt=torch.bfloat16, dev=dev)
+    a_rows = torch.arange(rows, device=dev)
+    a_rows[4], a_rows[21] = -1, rows
+    off = torch.tensor([2, 10, 10, 30], device=dev)
+
+    def go(off):
+        y = torch.full((rows, n), 7., dtype=torch.bfloat16, device=dev)
+        N.call('lcq_int4_gemm_grouped', N.ptr(x), N.BF16, k, rows, N.ptr(a_rows), rows,
+               N.ptr(off), N.ptr(tab), 3, 1, 0, 0, 128, n, k, N.ptr(y), N.stream_of(x))
+        return y
+    y = go(off)
+    assert (y[:2] == 7).all() and (y[30:] == 7).all()
+    assert (y[4] == 0).all() and (y[21] == 0).all()
+    for e, (a, b) in ((0, (2, 10)), (2, (10, 30))):
+        keep = [i for i in range(a, b) if i not in (4, 21)]
+        assert R.close(y[keep], *R.linear(x[keep], *ws[e]))
+    z = go(torch.tensor([-5, 10, 1 << 40, 3], device=dev))
+    assert R.close(z[10:21], *R.linear(x[10:21], *ws[1]))
+
+
+def test_other_stream_and_graph(dev):
+    """On a side stream, and captured into a graph that is replayed on new inputs."""
+    from lightcompress_amd import ops
+    g = torch.Generator().manual_seed(4)
+    for m in (2, 90):
+        w = weight(g, 'autoawq', 256, 1024, 128, dev)
+        x = acts(g, m, 1024, dt=torch.bfloat16, dev=dev)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            a = ops.int4_linear(x, *w)
+        torch.cuda.current_stream().wait_stream(s)
+        assert torch.equal(a, ops.int4_linear(x, *w))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.int4_linear(x, *w)
+        for _ in range(3):
+            x.copy_(acts(g, m, 1024, dt=torch.bfloat16, dev=dev))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, ops.int4_linear(x, *w))
