@@ -744,6 +744,46 @@ int lcq_int4_gemm_grouped(const void* x, int dtype, int64_t ldx, int64_t x_rows,
                           const int64_t* wtab, int64_t G, int nsets, int silu_mul, int layout,
                           int64_t group, int64_t n, int64_t k, void* y, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Latent attention of the DeepSeek-V3 adapter (models/deepseekv3.py; the checkpoint's modeling
+ * code and transformers' DeepseekV3Attention run it through sdpa on concatenated keys). Head
+ * dims are fixed: 128 nope + 64 rotary, values 128, latent 512. bf16 / fp16; strides in elements
+ * (host int64 arrays, last dim contiguous), multiples of 8; all tensors 16-byte aligned.
+ *
+ * Expanded, causal: out[b, i, h] = sum_j softmax_j((q_nope_i . k_nope_j + q_rope_i . k_rope_j)
+ * scale) v_j over the keys j <= q_start[b] + i, j < kv_lens[b]; a row without a key is zero.
+ * q_nope [B, H, Sq, 128], q_rope [B, H, Sq, 64], k_nope, v [B, H, Skv, 128]: strides {batch, head,
+ * seq}; k_rope [B, Skv, 64], shared by the heads: strides {batch, seq}. q_start int32 [B] (device;
+ * NULL: Skv - Sq), kv_lens int32 [B] (device; NULL: Skv; clamped to [0, Skv]). Keys at or past
+ * kv_lens are not read; those below must be finite (a NaN or an infinity there can reach rows that
+ * do not see the key). out [B, Sq, H, 128] contiguous. Key / value seq strides in [0, 2^24).
+ * ------------------------------------------------------------------------------------- */
+int lcq_mla_fwd_causal(const void* q_nope, const int64_t* q_nope_strides, const void* q_rope,
+                       const int64_t* q_rope_strides, const void* k_nope,
+                       const int64_t* k_nope_strides, const void* k_rope,
+                       const int64_t* k_rope_strides, const void* v, const int64_t* v_strides,
+                       int dtype, int64_t B, int64_t H, int64_t Sq, int64_t Skv,
+                       const int32_t* q_start, const int32_t* kv_lens, float scale, void* out,
+                       void* stream);
+
+/* Absorbed, over a paged latent cache (decode): out[b, i, h] = sum_j softmax_j((q_latent_i . c_j +
+ * q_rope_i . r_j) scale) c_j (512 dims) over the cached tokens j <= kv_lens[b] - Sq + i. Token j
+ * of sequence b is slot j % page_size of page block_table[b, j / page_size] (int32 [B, nb]). ckv
+ * [pages, page_size, 512], k_rope [pages, page_size, 64]: strides {page, slot}. q_latent
+ * [B, Sq, H, 512], q_rope [B, Sq, H, 64]: strides {batch, token, head}. kv_lens int32 [B] (clamped
+ * to [0, nb * page_size]) counts the Sq new tokens, which are in the cache already. A page number
+ * outside [0, pages) hides its tokens; a row without a token is zero; slots past a length are not
+ * read. out [B, Sq, H, 512] contiguous. workspace: lcq_mla_decode_workspace_bytes(B, Sq, H, nb *
+ * page_size) bytes (partial outputs of sequences that several workgroups share; joined in a fixed
+ * order: the same call gives the same bits). */
+int64_t lcq_mla_decode_workspace_bytes(int64_t B, int64_t Sq, int64_t H, int64_t max_len);
+int lcq_mla_decode(const void* q_latent, const int64_t* q_latent_strides, const void* q_rope,
+                   const int64_t* q_rope_strides, const void* ckv, const int64_t* ckv_strides,
+                   const void* k_rope, const int64_t* k_rope_strides, int64_t pages,
+                   int64_t page_size, const int32_t* block_table, int64_t nb,
+                   const int32_t* kv_lens, int dtype, int64_t B, int64_t Sq, int64_t H,
+                   float scale, void* out, void* workspace, int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1544,3 +1544,106 @@ def int4_linear_grouped(x: torch.Tensor, row_off: torch.Tensor, wtab: torch.Tens
                INT4_LAYOUTS[layout], int(group), int(n), k, N.ptr(y), N.stream_of(x2))
     N.note_work('lcq_int4_gemm_grouped', 2.0 * rows * n * k * nsets)
     return y
+
+
+# ---------------------------------------------------------------------------------------
+# latent attention (DeepSeek-V3): expanded for prompts, absorbed for decode
+# ---------------------------------------------------------------------------------------
+MLA_NOPE, MLA_ROPE, MLA_V, MLA_LATENT = 128, 64, 128, 512
+
+
+def _mla_rows(name, t, shape):
+    """t with 16-byte readable rows of `shape`; a copy where its strides or address do not fit."""
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f'{name} must be {list(shape)}, got {list(t.shape)}')
+    if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1]) or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _mla_checked(ref, dtype_of, **index):
+    for name, t in dtype_of.items():
+        if t.dtype != ref.dtype:
+            raise TypeError(f'{name} is {t.dtype}, not {ref.dtype}')
+    if ref.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f'bf16 / fp16 only, got {ref.dtype}')
+    for name, t in index.items():
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+            raise TypeError(f'{name} must be a contiguous int32 tensor')
+    _same_device(ref, **dtype_of, **index)
+
+
+def _strides(t, n):
+    import ctypes
+    return (ctypes.c_int64 * n)(*t.stride()[:n])
+
+
+def mla_fwd_causal(q_nope: torch.Tensor, q_rope: torch.Tensor, k_nope: torch.Tensor,
+                   k_rope: torch.Tensor, v: torch.Tensor, scale: float,
+                   q_start: torch.Tensor | None = None, kv_lens: torch.Tensor | None = None
+                   ) -> torch.Tensor:
+    """Latent attention in its expanded form, causal. q_nope [B, H, Sq, 128], q_rope
+    [B, H, Sq, 64], k_nope / v [B, H, Skv, 128] in any strides with a contiguous last dim (the
+    projections seen head by head), k_rope [B, Skv, 64] or [B, 1, Skv, 64], one rotary key for all
+    heads. Query i stands at position q_start[b] + i (int32 [B]; default Skv - Sq, the queries are
+    the last tokens) and sees the keys up to its position below kv_lens[b] (int32 [B]; default
+    Skv); a query that sees none gives zeros. Returns [B, Sq, H, 128] contiguous."""
+    B, H, Sq, _ = q_nope.shape
+    Skv = k_nope.shape[2]
+    if k_rope.dim() == 4 and k_rope.shape[1] == 1:
+        k_rope = k_rope[:, 0]
+    _mla_checked(q_nope, dict(q_rope=q_rope, k_nope=k_nope, k_rope=k_rope, v=v),
+                 q_start=q_start, kv_lens=kv_lens)
+    if any(t is not None and tuple(t.shape) != (B,) for t in (q_start, kv_lens)):
+        raise ValueError(f'q_start / kv_lens must have {B} entries')
+    qn = _mla_rows('q_nope', q_nope, (B, H, Sq, MLA_NOPE))
+    qr = _mla_rows('q_rope', q_rope, (B, H, Sq, MLA_ROPE))
+    kn = _mla_rows('k_nope', k_nope, (B, H, Skv, MLA_NOPE))
+    kr = _mla_rows('k_rope', k_rope, (B, Skv, MLA_ROPE))
+    vv = _mla_rows('v', v, (B, H, Skv, MLA_V))
+    out = torch.empty((B, Sq, H, MLA_V), dtype=qn.dtype, device=qn.device)
+    with N.on_device(qn):
+        N.call('lcq_mla_fwd_causal', N.ptr_strided(qn), _strides(qn, 3), N.ptr_strided(qr),
+               _strides(qr, 3), N.ptr_strided(kn), _strides(kn, 3), N.ptr_strided(kr),
+               _strides(kr, 2), N.ptr_strided(vv), _strides(vv, 3), N.dt(qn), B, H, Sq, Skv,
+               N.ptr(q_start), N.ptr(kv_lens), float(scale), N.ptr(out), N.stream_of(qn))
+    N.note_work('lcq_mla_fwd_causal',
+                2.0 * B * H * Sq * (Skv - (Sq - 1) / 2) * (MLA_NOPE + MLA_ROPE + MLA_V))
+    return out
+
+
+def mla_decode(q_latent: torch.Tensor, q_rope: torch.Tensor, ckv: torch.Tensor,
+               k_rope: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
+               scale: float) -> torch.Tensor:
+    """Latent attention in its absorbed form over a paged cache, for one or a few new tokens per
+    sequence. q_latent [B, Sq, H, 512] (the nope query times the key up-projection), q_rope
+    [B, Sq, H, 64]; ckv [pages, page_size, 512] and k_rope [pages, page_size, 64] (two views of
+    one cache, or two caches; any strides with a contiguous last dim); block_table int32 [B, nb]
+    names the pages of each sequence, kv_lens int32 [B] its tokens, the Sq new ones included: new
+    token i sees the first kv_lens - Sq + i + 1. A page number outside the cache hides its tokens;
+    a row that sees none gives zeros. Returns the attended latents [B, Sq, H, 512] contiguous."""
+    B, Sq, H, _ = q_latent.shape
+    P, ps = ckv.shape[:2]
+    _mla_checked(q_latent, dict(q_rope=q_rope, ckv=ckv, k_rope=k_rope), block_table=block_table,
+                 kv_lens=kv_lens)
+    if block_table.dim() != 2 or block_table.shape[0] != B or tuple(kv_lens.shape) != (B,):
+        raise ValueError(f'block_table must be [{B}, nb] and kv_lens [{B}]')
+    if P == 0 or ps == 0 or block_table.shape[1] == 0:
+        raise ValueError('empty cache')
+    ql = _mla_rows('q_latent', q_latent, (B, Sq, H, MLA_LATENT))
+    qr = _mla_rows('q_rope', q_rope, (B, Sq, H, MLA_ROPE))
+    for name, t, d in (('ckv', ckv, MLA_LATENT), ('k_rope', k_rope, MLA_ROPE)):
+        if tuple(t.shape) != (P, ps, d):
+            raise ValueError(f'{name} must be [{P}, {ps}, {d}], got {list(t.shape)}')
+        if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+            raise ValueError(f'{name} rows must be contiguous and 16-byte aligned')
+    nb = block_table.shape[1]
+    out = torch.empty((B, Sq, H, MLA_LATENT), dtype=ql.dtype, device=ql.device)
+    wsb = int(N.load().lcq_mla_decode_workspace_bytes(B, Sq, H, nb * ps))
+    ws = torch.empty(wsb, dtype=torch.uint8, device=ql.device) if wsb else None
+    with N.on_device(ql):
+        N.call('lcq_mla_decode', N.ptr_strided(ql), _strides(ql, 3), N.ptr_strided(qr),
+               _strides(qr, 3), N.ptr_strided(ckv), _strides(ckv, 2), N.ptr_strided(k_rope),
+               _strides(k_rope, 2), P, ps, N.ptr(block_table), nb, N.ptr(kv_lens), N.dt(ql), B,
+               Sq, H, float(scale), N.ptr(out), N.ptr(ws), wsb, N.stream_of(ql))
+    return out
