@@ -223,6 +223,9 @@ def stream_of(t: torch.Tensor):
 def on_device(t: torch.Tensor):
     """Context in which t's device is the current one (a launch on another device's stream is an
     error); does nothing where it already is."""
+    if not t.is_cuda:
+        raise LcqError('lightcompress_amd ops run on the GPU only (no CPU fallback); '
+                       f'got a tensor on {t.device}')
     if t.device.index == torch.cuda.current_device():
         return contextlib.nullcontext()
     return torch.cuda.device(t.device)

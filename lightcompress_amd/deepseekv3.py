@@ -12,6 +12,8 @@ and deploy. Block-fp8 checkpoints (``torch_dtype: torch.float8_e4m3fn``,
 """
 from __future__ import annotations
 
+import types
+
 import torch
 import torch.nn as nn
 
@@ -32,6 +34,9 @@ class ExpertList(nn.ModuleList):
         if (top_k_weights.dtype in (torch.float32, torch.bfloat16, torch.float16)
                 and self._grouped_fp8_ok(hidden_states)):
             return self._forward_grouped_fp8(hidden_states, top_k_index, top_k_weights)
+        if (top_k_weights.dtype in (torch.float32, torch.bfloat16, torch.float16)
+                and self._grouped_int4_ok(hidden_states)):
+            return self._forward_grouped_int4(hidden_states, top_k_index, top_k_weights)
         out = torch.zeros_like(hidden_states)
         with torch.no_grad():
             mask = torch.nn.functional.one_hot(top_k_index, num_classes=len(self)).permute(2, 1, 0)
@@ -57,9 +62,9 @@ class ExpertList(nn.ModuleList):
     # epilogue as the MLP computes it on the bf16 projections; one launch for down, then lcq_moe_combine in the loop's order (per token, experts in
     # ascending index, each product rounded to bf16 before its add, as index_add_ does).
     # Every row's GEMM value equals lcq_fp8_gemm's on an unsplit 256^2 plan.
-    def _grouped_fp8_ok(self, x) -> bool:
-        from .module_utils import USE_FP8GEMM_TRITON_KERNEL, LlmcFp8Linear
-        if (not USE_FP8GEMM_TRITON_KERNEL or not len(self) or x.dim() != 2 or not x.is_cuda
+    def _plain_mlps(self, x) -> bool:
+        """x fits the grouped kernels and every expert is the stock MLP with no hooks."""
+        if (not len(self) or x.dim() != 2 or not x.is_cuda
                 or x.dtype != torch.bfloat16 or len(self) > 1 << 20
                 or torch.nn.modules.module._global_forward_hooks
                 or torch.nn.modules.module._global_forward_pre_hooks):
@@ -71,6 +76,13 @@ class ExpertList(nn.ModuleList):
             for m in (mlp, mlp.gate_proj, mlp.up_proj, mlp.down_proj):
                 if m._forward_hooks or m._forward_pre_hooks:
                     return False
+        return True
+
+    def _grouped_fp8_ok(self, x) -> bool:
+        from .module_utils import USE_FP8GEMM_TRITON_KERNEL, LlmcFp8Linear
+        if not USE_FP8GEMM_TRITON_KERNEL or not self._plain_mlps(x):
+            return False
+        for mlp in self:
             for lin in (mlp.gate_proj, mlp.up_proj, mlp.down_proj):
                 if (type(lin) is not LlmcFp8Linear or lin.bias is not None
                         or lin.block_size != 128 or lin.weight.dtype != torch.float8_e4m3fn
@@ -132,6 +144,71 @@ class ExpertList(nn.ModuleList):
         w = top_k_weights if top_k_weights.dtype != torch.float16 else top_k_weights.float()
         return ops.moe_combine(y, slot_row, top_k_index.to(torch.int64), w, T)
 
+
+    # ---- packed 4-bit experts (a deployed vLLM / AutoAWQ model) -----------------------------
+    # Same shape as the fp8 path on lcq_int4_gemm_grouped: one launch for gate and up of every
+    # expert with the SiLU product in its epilogue (in fp32: one rounding where the per-expert
+    # modules round gate, up, silu and the product), one for down, lcq_moe_combine. Nothing is read
+    # on the host, so a decode step can be captured.
+    def _grouped_int4_ok(self, x) -> bool:
+        from .module_utils import int4_weight
+        if not self._plain_mlps(x) or getattr(self[0].config, 'hidden_act', None) != 'silu':
+            return False
+        for p in ('gate_proj', 'up_proj', 'down_proj'):
+            kinds = set()
+            for mlp in self:
+                w = int4_weight(getattr(mlp, p))
+                if w is None or w[0].device != x.device:
+                    return False
+                kinds.add((w[2] is None, tuple(w[0].shape), tuple(w[1].shape)))
+            if len(kinds) != 1:
+                return False
+        gate, up = int4_weight(self[0].gate_proj), int4_weight(self[0].up_proj)
+        return (gate[2] is None) == (up[2] is None) and gate[1].shape == up[1].shape
+
+    def _int4_tables(self, device):
+        """([2, E, 3] gate + up, [E, 3] down) device tables of the experts' packed buffers,
+        rebuilt when any of them changed (the modules keep the tensors)."""
+        from . import ops
+        from .module_utils import int4_weight
+        ws = [[int4_weight(getattr(mlp, p)) for mlp in self]
+              for p in ('gate_proj', 'up_proj', 'down_proj')]
+        key = tuple(None if t is None else t.data_ptr() for row in ws for w in row for t in w)
+        cached = getattr(self, '_lcq_int4_tables', None)
+        if cached is None or cached[0] != key:
+            gate, up, down = (ops.int4_weight_table(row, device) for row in ws)
+            cached = (key, (torch.stack([gate, up]).contiguous(), down))
+            self._lcq_int4_tables = cached
+        return cached[1]
+
+    def _forward_grouped_int4(self, hidden_states, top_k_index, top_k_weights):
+        from . import ops
+        from .module_utils import int4_weight
+        T, k = top_k_index.shape
+        E, H = len(self), hidden_states.shape[1]
+        if T == 0:
+            return torch.zeros_like(hidden_states)
+        gate_up, down = self._int4_tables(hidden_states.device)
+        inter = self[0].gate_proj.out_features
+
+        def kind(lin):
+            _, s, z = int4_weight(lin)
+            return (lin.in_features // s.shape[1 if z is None else 0],
+                    'vllm' if z is None else 'autoawq')
+        with torch.no_grad():
+            flat, order = torch.sort(top_k_index.reshape(-1).to(torch.int64), stable=True)
+            row_off = torch.searchsorted(flat, torch.arange(E + 1, device=flat.device))
+            slot_row = torch.empty_like(order)                # (token, slot) -> sorted row
+            slot_row[order] = torch.arange(order.numel(), device=order.device)
+        g, layout = kind(self[0].gate_proj)
+        h = ops.int4_linear_grouped(hidden_states, row_off, gate_up, inter, g, layout,
+                                    a_rows=order // k, silu_mul=True)
+        g, layout = kind(self[0].down_proj)
+        y = ops.int4_linear_grouped(h, row_off, down, H, g, layout)
+        w = top_k_weights if top_k_weights.dtype != torch.float16 else top_k_weights.float()
+        return ops.moe_combine(y, slot_row, top_k_index.to(torch.int64), w, T)
+
+
 def _mlp_forward():
     try:
         from transformers.models.deepseek_v3 import modeling_deepseek_v3 as md
@@ -169,6 +246,83 @@ def unfuse_experts(model: nn.Module) -> nn.Module:
     return model
 
 
+def _plain_weight(lin):
+    """The weight of a linear that is exactly x W^T with no hooks, None for anything else."""
+    from .llama import _linear_wb
+    wb = _linear_wb(lin)
+    if wb is None or wb[1] is not None or lin._forward_hooks or lin._forward_pre_hooks:
+        return None
+    return wb[0]
+
+
+def _lcq_mla_ok(attn, x, attention_mask, past_key_values, kwargs) -> bool:
+    """The cases the lcq latent attention takes: causal without a mask (a prompt with no cached
+    tokens, or one new token), no dropout or attention weights asked for, the checkpoint's head
+    dims, bf16 / fp16 on the device, no autograd."""
+    if (not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float16) or x.dim() != 3
+            or attention_mask is not None or kwargs.get('output_attentions')
+            or kwargs.get('is_causal') is False
+            or (attn.training and attn.attention_dropout)
+            or (torch.is_grad_enabled() and any(p.requires_grad for p in attn.parameters()))
+            or attn.config._attn_implementation != 'sdpa'
+            or (attn.qk_nope_head_dim, attn.qk_rope_head_dim, attn.v_head_dim,
+                attn.kv_lora_rank) != (128, 64, 128, 512)):
+        return False
+    past = past_key_values.get_seq_length(attn.layer_idx) if past_key_values is not None else 0
+    return past == 0 or x.shape[1] == 1
+
+
+def _lcq_mla_forward(self, hidden_states, position_embeddings, attention_mask,
+                     past_key_values=None, **kwargs):
+    """DeepseekV3Attention.forward on the lcq latent attention: prompts in the expanded form on
+    kv_b_proj's own output (no concatenated keys), one new token behind cached latents in the
+    absorbed form (no up-projection of the cache) where kv_b_proj is a plain weight. Anything
+    _lcq_mla_ok does not take runs the stock forward."""
+    from transformers.models.deepseek_v3 import modeling_deepseek_v3 as md
+
+    from . import ops
+    if not _lcq_mla_ok(self, hidden_states, attention_mask, past_key_values, kwargs):
+        return type(self).forward(self, hidden_states, position_embeddings, attention_mask,
+                                  past_key_values, **kwargs)
+    B, S = hidden_states.shape[:2]
+    H = self.num_heads
+    if self.q_lora_rank is None:
+        q = self.q_proj(hidden_states)
+    else:
+        q = self.q_b_proj(self.q_a_layernorm(self.q_a_proj(hidden_states)))
+    q = q.view(B, S, H, self.qk_head_dim).transpose(1, 2)
+    q_nope, q_rot = q.split([self.qk_nope_head_dim, self.qk_rope_head_dim], dim=-1)
+    ckv, k_rot = self.kv_a_proj_with_mqa(hidden_states).split(
+        [self.kv_lora_rank, self.qk_rope_head_dim], dim=-1)
+    ckv = self.kv_a_layernorm(ckv).view(B, 1, S, self.kv_lora_rank)
+    k_rot = k_rot.view(B, 1, S, self.qk_rope_head_dim)
+    cos, sin = position_embeddings
+    rope = (md.apply_rotary_pos_emb_interleave if self.config.rope_interleave
+            else md.apply_rotary_pos_emb)
+    q_rot, k_rot = rope(q_rot, k_rot, cos, sin)
+    if past_key_values is not None:
+        ckv, k_rot = past_key_values.update(ckv, k_rot, self.layer_idx)
+    T = ckv.shape[2]
+    w = _plain_weight(self.kv_b_proj) if T > S else None
+    if w is not None and w.dtype == q.dtype:
+        # one new token: q_latent = q_nope W_k per head, the attended latent times W_v^T
+        w = w.view(H, -1, self.kv_lora_rank)
+        wk, wv = w[:, :self.qk_nope_head_dim], w[:, self.qk_nope_head_dim:]
+        qn = q_nope.permute(1, 0, 2, 3).reshape(H, B * S, -1)
+        ql = torch.bmm(qn, wk).view(H, B, S, -1).permute(1, 2, 0, 3)
+        dev = ckv.device
+        lat = ops.mla_decode(ql, q_rot.transpose(1, 2), ckv[:, 0], k_rot[:, 0],
+                             torch.arange(B, dtype=torch.int32, device=dev)[:, None],
+                             torch.full((B,), T, dtype=torch.int32, device=dev), self.scaling)
+        out = torch.bmm(wv, lat.view(B * S, H, -1).permute(1, 2, 0).contiguous())
+        out = out.view(H, -1, B, S).permute(2, 3, 0, 1)
+    else:
+        kv = self.kv_b_proj(ckv.squeeze(1)).view(B, T, H, -1).transpose(1, 2)
+        k_nope, v = kv.split([self.qk_nope_head_dim, self.v_head_dim], dim=-1)
+        out = ops.mla_fwd_causal(q_nope, q_rot, k_nope, k_rot, v, self.scaling)
+    return self.o_proj(out.reshape(B, S, -1)), None
+
+
 @MODEL_REGISTRY
 class DeepseekV3(BaseModel):
     block_name_prefix = 'model.layers'
@@ -180,7 +334,19 @@ class DeepseekV3(BaseModel):
         # LlmcFp8Linear modules (BaseModel.load_checkpoint)
         self.block_fp8 = td in ('torch.float8_e4m3fn', 'float8_e4m3fn') or \
             dtype == torch.float8_e4m3fn
+        # attention of the forwards: 'sdpa' (transformers') or 'lcq' (_lcq_mla_forward)
+        self.attention = mcfg.get('attention', 'sdpa')
+        if self.attention not in ('sdpa', 'lcq'):
+            raise ValueError(f"model.attention must be 'sdpa' or 'lcq', got {self.attention!r}")
         super().__init__(config, hf_model=hf_model, device=device, dtype=dtype, **kw)
+
+    def install_fused_forward(self):
+        super().install_fused_forward()
+        if self.attention == 'lcq':
+            from transformers.models.deepseek_v3 import modeling_deepseek_v3 as md
+            for m in self.model.modules():
+                if type(m) is md.DeepseekV3Attention:
+                    m.forward = types.MethodType(_lcq_mla_forward, m)
 
     def prepare_model(self, hf_model):
         return unfuse_experts(hf_model)

@@ -269,8 +269,13 @@ def _staged_decoder_forward(self, hidden_states, attention_mask=None, position_i
     when its input, a module object or a weight (storage or in-place version) changed, and
     always when one of its modules carries hooks (so input captures keep firing)."""
     attn, mlp = self.self_attn, self.mlp
+    # (a deployed packed block runs the model, not the calibration: nothing is memoised, since
+    # fresh inputs of one decode step after another may share an address)
     if (past_key_values is not None or not hidden_states.is_cuda
-            or _hooked(self, attn, mlp)):
+            or _hooked(self, attn, mlp)
+            or any(hasattr(m, 'int4_forward') for m in (
+                attn.q_proj, attn.k_proj, attn.v_proj, attn.o_proj, mlp.gate_proj, mlp.up_proj,
+                mlp.down_proj))):
         return _STOCK_DECODER_FORWARD(self, hidden_states, attention_mask=attention_mask,
                                       position_ids=position_ids,
                                       past_key_values=past_key_values, use_cache=use_cache,

@@ -238,8 +238,24 @@ def _module_shell(cls, buffers: dict, attrs: dict):
     return m
 
 
+def _int4_forward(quant_config, bits_ok: bool) -> bool:
+    """A packed linear can compute its own product (ops.int4_linear): 4-bit codes whose scales
+    (and zero points) it holds, weight-only -- with an `act` section the deployed product takes
+    quantized activations, which this one does not."""
+    return bits_ok and quant_config.get('act') is None
+
+
+def _vllm_int4(quant_config) -> bool:
+    w = quant_config['weight']
+    return _int4_forward(quant_config, bool(
+        w.get('need_pack', False) and w.get('bit') == 4 and w.get('symmetric')
+        and w.get('granularity') in ('per_group', 'per_channel')))
+
+
 class VllmRealQuantLinear(nn.Module):
-    """module_utils.py:855-955 — vLLM compressed-tensors int layout."""
+    """module_utils.py:855-955 — vLLM compressed-tensors int layout. The reference's forward
+    raises; here a weight-only module of packed symmetric 4-bit codes (``int4_forward``) computes
+    its product from the packed words."""
 
     def __init__(self, weight, bias, scales, input_scale, need_pack, scales_name):
         super().__init__()
@@ -250,10 +266,13 @@ class VllmRealQuantLinear(nn.Module):
             self.bias = None
         self.register_buffer(scales_name, scales)
         self.register_buffer('input_scale', input_scale)
+        self.int4_forward = False
 
     @torch.no_grad()
     def forward(self, x):
-        raise NotImplementedError
+        if not self.int4_forward:
+            raise NotImplementedError('only weight-only packed symmetric 4-bit weights run here')
+        return ops.int4_linear(x, self.weight_packed, self.weight_scale, bias=self.bias)
 
     @classmethod
     @torch.no_grad()
@@ -269,6 +288,7 @@ class VllmRealQuantLinear(nn.Module):
         m.weight_shape, m.weight_dtype = weight.shape, weight.dtype
         m.scales_shape, m.scales_dtype = scales.shape, scales.dtype
         m.zeros_shape = m.zeros_dtype = None
+        m.int4_forward = _vllm_int4(quant_config)
         return m
 
     @classmethod
@@ -284,6 +304,7 @@ class VllmRealQuantLinear(nn.Module):
         scales_name = ('weight_scale_inv' if quant_config['weight']['granularity'] == 'per_block'
                        else 'weight_scale')
         wname = 'weight_packed' if need_pack else 'weight'
+        int4 = _vllm_int4(quant_config)
         out = []
         for i, module in enumerate(modules):
             pre = prequant[i] if prequant is not None else None
@@ -300,7 +321,7 @@ class VllmRealQuantLinear(nn.Module):
             attrs.update(in_features=module.in_features, out_features=module.out_features,
                          weight_shape=weight.shape, weight_dtype=weight.dtype,
                          scales_shape=scales.shape, scales_dtype=scales.dtype,
-                         zeros_shape=None, zeros_dtype=None)
+                         zeros_shape=None, zeros_dtype=None, int4_forward=int4)
             out.append(_module_shell(cls, bufs, attrs))
         return out
 
@@ -346,7 +367,8 @@ class Lightx2vRealQuantLinear(VllmRealQuantLinear):
 
 
 class AutoawqRealQuantLinear(nn.Module):
-    """module_utils.py:1025-1158 — AutoAWQ GEMM layout (qweight [IC, OC/8])."""
+    """module_utils.py:1025-1158 — AutoAWQ GEMM layout (qweight [IC, OC/8]). The reference's
+    forward raises; here a weight-only module computes its product from the packed words."""
 
     def __init__(self, weight, bias, scales, zeros):
         super().__init__()
@@ -360,10 +382,13 @@ class AutoawqRealQuantLinear(nn.Module):
             self.register_buffer('qzeros', zeros)
         else:
             self.qzeros = None
+        self.int4_forward = False
 
     @torch.no_grad()
     def forward(self, x):
-        raise NotImplementedError
+        if not self.int4_forward:
+            raise NotImplementedError('only weight-only packed 4-bit weights run here')
+        return ops.int4_linear(x, self.qweight, self.scales, self.qzeros, self.bias)
 
     @classmethod
     @torch.no_grad()
@@ -376,6 +401,7 @@ class AutoawqRealQuantLinear(nn.Module):
         m.scales_shape, m.scales_dtype = scales.shape, scales.dtype
         m.zeros_shape = zeros.shape if zeros is not None else None
         m.zeros_dtype = zeros.dtype if zeros is not None else None
+        m.int4_forward = _int4_forward(quant_config, zeros is not None)
         return m
 
     @classmethod
@@ -414,6 +440,16 @@ _REALQUANT_LINEAR_MAP_ = {
     'mlcllm_quant': MlcllmRealQuantLinear,
     'lightx2v_quant': Lightx2vRealQuantLinear,
 }
+
+def int4_weight(m):
+    """(qweight, scales, qzeros | None) of a packed linear that runs its own product (with no
+    bias), None for anything else."""
+    if not getattr(m, 'int4_forward', False) or m.bias is not None:
+        return None
+    if isinstance(m, AutoawqRealQuantLinear):
+        return m.qweight, m.scales, m.qzeros
+    return m.weight_packed, m.weight_scale, None
+
 
 _LLMC_LINEAR_TYPES_ = [LlmcFp8Linear, OriginFloatLinear, FakeQuantLinear,
                        EffcientFakeQuantLinear, VllmRealQuantLinear, SglRealQuantLinear,
