@@ -725,11 +725,15 @@ int lcq_gemm_sq_diff(const void* a, int dtype, int64_t lda, int64_t m, int64_t k
  * (row stride ldy) in the same dtype. group % 32 == 0, k % group == 0, layout 1: n % 8 == 0; any
  * m >= 0 (0: nothing to do). Codes and zero points enter exactly, sums are fp32 (a fixed order:
  * the same call gives the same bits), one rounding at the end. A row of x with an infinity or a
- * NaN gives NaN in that row.
+ * NaN gives NaN in that row. n k < 2^32, k < 2^21. workspace:
+ * lcq_int4_gemm_workspace_bytes(m, n, k, layout) bytes (partial sums of a long k split over
+ * workgroups; 0 where none is needed).
  * ------------------------------------------------------------------------------------- */
+int64_t lcq_int4_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int layout);
 int lcq_int4_gemm(const void* x, int dtype, int64_t ldx, int64_t m, int64_t k,
                   const void* qweight, const void* scales, const void* qzeros, int layout,
-                  int64_t group, int64_t n, const void* bias, void* y, int64_t ldy, void* stream);
+                  int64_t group, int64_t n, const void* bias, void* y, int64_t ldy,
+                  void* workspace, int64_t ws_bytes, void* stream);
 
 /* lcq_int4_gemm for the G routed experts of an MoE projection in one launch (the expert loop of
  * the reference's models/deepseekv3.py MoE forward on packed experts). Rows and groups as in

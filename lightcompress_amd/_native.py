@@ -144,8 +144,9 @@ SIGNATURES = {
     'lcq_gemm_sq_diff_workspace_bytes': ([_i64, _i64], _i64),
     'lcq_gemm_sq_diff': ([_vp, _int, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp,
                           _i64, _vp, _int, _vp], _int),
+    'lcq_int4_gemm_workspace_bytes': ([_i64, _i64, _i64, _int], _i64),
     'lcq_int4_gemm': ([_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _int, _i64, _i64, _vp, _vp,
-                       _i64, _vp], _int),
+                       _i64, _vp, _i64, _vp], _int),
     'lcq_int4_gemm_grouped': ([_vp, _int, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _int, _int,
                                _int, _i64, _i64, _i64, _vp, _vp], _int),
     'lcq_mla_fwd_causal': ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64,
@@ -217,7 +218,11 @@ def ptr_strided(t):
 
 
 def stream_of(t: torch.Tensor):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # torch.cuda.current_stream(t.device).cuda_stream without building the Stream object
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+_HERE = contextlib.nullcontext()
 
 
 def on_device(t: torch.Tensor):
@@ -226,8 +231,8 @@ def on_device(t: torch.Tensor):
     if not t.is_cuda:
         raise LcqError('lightcompress_amd ops run on the GPU only (no CPU fallback); '
                        f'got a tensor on {t.device}')
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if t.get_device() == torch._C._cuda_getDevice():
+        return _HERE
     return torch.cuda.device(t.device)
 
 

@@ -9,7 +9,7 @@
 // 16 costs at most 2 more bits of the fp32 sum than a signed code would.
 #pragma once
 
-#include "lcq_common.h"
+#include "lds_dma.h"
 
 namespace lcq {
 
@@ -50,12 +50,44 @@ __device__ __forceinline__ i4_v4u i4_word(uint32_t w) {
   return i4_v4u{i4_pair<DT, 0>(w), i4_pair<DT, 1>(w), i4_pair<DT, 2>(w), i4_pair<DT, 3>(w)};
 }
 
+// nibble t of every half of four packed pairs
+template <int DT>
+__device__ __forceinline__ i4_v4u i4_nibble(i4_v4u v, int t) {
+  auto f = [&](uint32_t w) {
+    return t == 0 ? i4_pair<DT, 0>(w) : t == 1 ? i4_pair<DT, 1>(w) : t == 2 ? i4_pair<DT, 2>(w)
+                                                                           : i4_pair<DT, 3>(w);
+  };
+  return i4_v4u{f(v.x), f(v.y), f(v.z), f(v.w)};
+}
+
 // 8 consecutive x values as an A fragment in that order
 __device__ __forceinline__ i4_v4u i4_xorder(i4_v4u d) {
   return i4_v4u{__builtin_amdgcn_perm(d.z, d.x, 0x05040100u),
                 __builtin_amdgcn_perm(d.z, d.x, 0x07060302u),
                 __builtin_amdgcn_perm(d.w, d.y, 0x05040100u),
                 __builtin_amdgcn_perm(d.w, d.y, 0x07060302u)};
+}
+
+// AutoAWQ words hold 8 columns of one k: 16 bits of a word are 4 columns. Four B fragments (4
+// tiles, 64 columns) come from two transposed LDS reads (ds_read_b64_tr_b16) of the words as they
+// lie: lane c of a 16-lane group gets 16-bit column c of 4 rows (k) each, in packed pairs. Its
+// tile t is nibble t of them: column 8 (c / 2) + 2 t + c % 2.
+__device__ __forceinline__ int i4_awq_column(int c, int t) { return 8 * (c >> 1) + 2 * t + (c & 1); }
+
+// XOR of the 16-byte chunks of 256-byte LDS rows: conflict-free for 16 rows at one chunk
+__device__ __forceinline__ int i4_swz(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
+
+// 4 x 4 transpose of words between the lanes q = 0..3 of a row (lane = 16 q + row)
+__device__ __forceinline__ i4_v4u i4_transpose(i4_v4u v) {
+  auto p = __builtin_amdgcn_permlane32_swap(v.x, v.z, false, false);
+  v.x = p[0]; v.z = p[1];
+  p = __builtin_amdgcn_permlane32_swap(v.y, v.w, false, false);
+  v.y = p[0]; v.w = p[1];
+  p = __builtin_amdgcn_permlane16_swap(v.x, v.y, false, false);
+  v.x = p[0]; v.y = p[1];
+  p = __builtin_amdgcn_permlane16_swap(v.z, v.w, false, false);
+  v.z = p[0]; v.w = p[1];
+  return v;
 }
 
 }  // namespace lcq

@@ -1414,46 +1414,51 @@ INT4_LAYOUTS = {'vllm': 0, 'autoawq': 1}
 
 
 def _same_device(ref: torch.Tensor, **tensors):
+    dev = ref.device
     for name, t in tensors.items():
-        if t is not None and t.device != ref.device:
-            raise ValueError(f'{name} is on {t.device}, not on {ref.device}')
+        if t is not None and t.device != dev:
+            raise ValueError(f'{name} is on {t.device}, not on {dev}')
 
 
 def _int4_weight(qweight, scales, qzeros):
     """(layout, n, k, group) of a packed weight after checking its tensors."""
-    layout = 'vllm' if qzeros is None else 'autoawq'
-    if qweight.dtype != torch.int32 or qweight.dim() != 2 or not qweight.is_contiguous():
+    if qweight.dtype is not torch.int32 or qweight.dim() != 2 or not qweight.is_contiguous():
         raise TypeError('qweight must be a contiguous 2-D int32 tensor')
-    if scales.dtype != torch.float16 or scales.dim() != 2 or not scales.is_contiguous():
+    if scales.dtype is not torch.float16 or scales.dim() != 2 or not scales.is_contiguous():
         raise TypeError('scales must be a contiguous 2-D fp16 tensor')
-    if layout == 'vllm':
-        n, k = qweight.shape[0], qweight.shape[1] * 8
-        ng, ns = scales.shape[1], scales.shape[0]
+    if qzeros is None:
+        layout = 'vllm'
+        n, k = qweight.shape
+        k *= 8
+        ns, ng = scales.shape
+        _same_device(qweight, scales=scales)
     else:
-        k, n = qweight.shape[0], qweight.shape[1] * 8
+        layout = 'autoawq'
+        k, n = qweight.shape
+        n *= 8
         ng, ns = scales.shape
-        if (qzeros.dtype != torch.int32 or not qzeros.is_contiguous()
-                or tuple(qzeros.shape) != (ng, n // 8)):
+        if (qzeros.dtype is not torch.int32 or not qzeros.is_contiguous()
+                or qzeros.shape != (ng, n // 8)):
             raise ValueError(f'qzeros must be contiguous int32 [{ng}, {n // 8}]')
-        _same_device(qweight, qzeros=qzeros)
+        _same_device(qweight, scales=scales, qzeros=qzeros)
     if n == 0 or k == 0 or ns != n or ng == 0 or k % ng:
         raise ValueError(f'scales {tuple(scales.shape)} do not fit a {layout} weight [{n}, {k}]')
     if (k // ng) % 32:
         raise ValueError(f'group size {k // ng} is not a multiple of 32')
-    _same_device(qweight, scales=scales)
-    if qweight.data_ptr() % 16 or scales.data_ptr() % 16:
+    if (qweight.data_ptr() | scales.data_ptr()) & 15:
         raise ValueError('packed weights and scales must be 16-byte aligned')
     return layout, n, k, k // ng
 
 
 def _int4_x(x: torch.Tensor, k: int) -> torch.Tensor:
     """x as rows the kernels can read: 2-D, rows 16-byte aligned, columns contiguous."""
-    if x.dtype not in (torch.bfloat16, torch.float16):
+    if x.dtype is not torch.bfloat16 and x.dtype is not torch.float16:
         raise TypeError(f'bf16 / fp16 activations only, got {x.dtype}')
     if x.dim() == 0 or x.shape[-1] != k:
         raise ValueError(f'x has {x.shape[-1] if x.dim() else 0} columns, the weight {k}')
     x2 = x if x.dim() == 2 else x.reshape(-1, k)
-    if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.stride(0) < k or x2.data_ptr() % 16:
+    ldx, one = x2.stride()
+    if one != 1 or ldx % 8 or ldx < k or x2.data_ptr() % 16:
         x2 = x2.clone(memory_format=torch.contiguous_format)
     return x2
 
@@ -1470,16 +1475,20 @@ def int4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
     to x's dtype. Not differentiable."""
     layout, n, k, group = _int4_weight(qweight, scales, qzeros)
     x2 = _int4_x(x, k)
-    _same_device(x2, qweight=qweight, bias=bias)
     if bias is not None and (bias.dtype != x.dtype or bias.dim() != 1 or bias.numel() != n
                              or not bias.is_contiguous()):
         raise ValueError(f'bias must be a contiguous [{n}] tensor in the dtype of x')
-    y = torch.empty((x2.shape[0], n), dtype=x.dtype, device=x2.device)
+    _same_device(x2, qweight=qweight, bias=bias)
+    m, lay = x2.shape[0], INT4_LAYOUTS[layout]
+    y = x2.new_empty((m, n))
+    wsb = N.load().lcq_int4_gemm_workspace_bytes(m, n, k, lay)
+    ws = x2.new_empty(wsb, dtype=torch.uint8) if wsb else None
     with N.on_device(x2):
-        N.call('lcq_int4_gemm', N.ptr_strided(x2), N.dt(x2), x2.stride(0), x2.shape[0], k,
-               N.ptr(qweight), N.ptr(scales), N.ptr(qzeros), INT4_LAYOUTS[layout], group, n,
-               N.ptr(bias), N.ptr(y), n, N.stream_of(x2))
-    N.note_work('lcq_int4_gemm', 2.0 * x2.shape[0] * n * k)
+        N.call('lcq_int4_gemm', x2.data_ptr(), N.dt(x2), x2.stride(0), m, k, qweight.data_ptr(),
+               scales.data_ptr(), None if qzeros is None else qzeros.data_ptr(), lay, group, n,
+               None if bias is None else bias.data_ptr(), y.data_ptr(), n,
+               None if ws is None else ws.data_ptr(), wsb, N.stream_of(x2))
+    N.note_work('lcq_int4_gemm', 2.0 * m * n * k)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
 
 
@@ -1536,12 +1545,12 @@ def int4_linear_grouped(x: torch.Tensor, row_off: torch.Tensor, wtab: torch.Tens
         raise ValueError('silu_mul takes the gate and up tables ([2, G, 3])')
     _same_device(x2, row_off=row_off, wtab=wtab, a_rows=a_rows)
     rows = x2.shape[0] if a_rows is None else a_rows.numel()
-    y = torch.empty((rows, n) if nsets == 1 or silu_mul else (nsets, rows, n), dtype=x.dtype,
-                    device=x2.device)
+    y = x2.new_empty((rows, n) if nsets == 1 or silu_mul else (nsets, rows, n))
     with N.on_device(x2):
-        N.call('lcq_int4_gemm_grouped', N.ptr_strided(x2), N.dt(x2), x2.stride(0), x2.shape[0],
-               N.ptr(a_rows), rows, N.ptr(row_off), N.ptr(wtab), G, nsets, int(bool(silu_mul)),
-               INT4_LAYOUTS[layout], int(group), int(n), k, N.ptr(y), N.stream_of(x2))
+        N.call('lcq_int4_gemm_grouped', x2.data_ptr(), N.dt(x2), x2.stride(0), x2.shape[0],
+               None if a_rows is None else a_rows.data_ptr(), rows, row_off.data_ptr(),
+               wtab.data_ptr(), G, nsets, int(bool(silu_mul)), INT4_LAYOUTS[layout], int(group),
+               int(n), k, y.data_ptr(), N.stream_of(x2))
     N.note_work('lcq_int4_gemm_grouped', 2.0 * rows * n * k * nsets)
     return y
 
@@ -1554,28 +1563,38 @@ MLA_NOPE, MLA_ROPE, MLA_V, MLA_LATENT = 128, 64, 128, 512
 
 def _mla_rows(name, t, shape):
     """t with 16-byte readable rows of `shape`; a copy where its strides or address do not fit."""
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f'{name} must be {list(shape)}, got {list(t.shape)}')
-    if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1]) or t.data_ptr() % 16:
+    st = t.stride()
+    if st[-1] != 1 or (st[0] | st[1] | (st[2] if len(st) == 4 else 0)) & 7 or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _mla_checked(ref, dtype_of, **index):
+    dt = ref.dtype
     for name, t in dtype_of.items():
-        if t.dtype != ref.dtype:
-            raise TypeError(f'{name} is {t.dtype}, not {ref.dtype}')
-    if ref.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f'bf16 / fp16 only, got {ref.dtype}')
+        if t.dtype is not dt:
+            raise TypeError(f'{name} is {t.dtype}, not {dt}')
+    if dt is not torch.bfloat16 and dt is not torch.float16:
+        raise TypeError(f'bf16 / fp16 only, got {dt}')
     for name, t in index.items():
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous()):
             raise TypeError(f'{name} must be a contiguous int32 tensor')
     _same_device(ref, **dtype_of, **index)
 
 
-def _strides(t, n):
+def _strides(*ts):
+    """(keep, pointers): the leading strides of each tensor (all dims but the last) in one host
+    int64 array."""
     import ctypes
-    return (ctypes.c_int64 * n)(*t.stride()[:n])
+    flat = [s for t in ts for s in t.stride()[:-1]]
+    keep = (ctypes.c_int64 * len(flat))(*flat)
+    at, out = ctypes.addressof(keep), []
+    for t in ts:
+        out.append(at)
+        at += 8 * (t.dim() - 1)
+    return keep, out
 
 
 def mla_fwd_causal(q_nope: torch.Tensor, q_rope: torch.Tensor, k_nope: torch.Tensor,
@@ -1601,12 +1620,14 @@ def mla_fwd_causal(q_nope: torch.Tensor, q_rope: torch.Tensor, k_nope: torch.Ten
     kn = _mla_rows('k_nope', k_nope, (B, H, Skv, MLA_NOPE))
     kr = _mla_rows('k_rope', k_rope, (B, Skv, MLA_ROPE))
     vv = _mla_rows('v', v, (B, H, Skv, MLA_V))
-    out = torch.empty((B, Sq, H, MLA_V), dtype=qn.dtype, device=qn.device)
+    out = qn.new_empty((B, Sq, H, MLA_V))
+    keep, st = _strides(qn, qr, kn, kr, vv)
     with N.on_device(qn):
-        N.call('lcq_mla_fwd_causal', N.ptr_strided(qn), _strides(qn, 3), N.ptr_strided(qr),
-               _strides(qr, 3), N.ptr_strided(kn), _strides(kn, 3), N.ptr_strided(kr),
-               _strides(kr, 2), N.ptr_strided(vv), _strides(vv, 3), N.dt(qn), B, H, Sq, Skv,
-               N.ptr(q_start), N.ptr(kv_lens), float(scale), N.ptr(out), N.stream_of(qn))
+        N.call('lcq_mla_fwd_causal', qn.data_ptr(), st[0], qr.data_ptr(), st[1], kn.data_ptr(),
+               st[2], kr.data_ptr(), st[3], vv.data_ptr(), st[4], N.dt(qn), B, H, Sq, Skv,
+               None if q_start is None else q_start.data_ptr(),
+               None if kv_lens is None else kv_lens.data_ptr(), float(scale), out.data_ptr(),
+               N.stream_of(qn))
     N.note_work('lcq_mla_fwd_causal',
                 2.0 * B * H * Sq * (Skv - (Sq - 1) / 2) * (MLA_NOPE + MLA_ROPE + MLA_V))
     return out
@@ -1633,17 +1654,19 @@ def mla_decode(q_latent: torch.Tensor, q_rope: torch.Tensor, ckv: torch.Tensor,
     ql = _mla_rows('q_latent', q_latent, (B, Sq, H, MLA_LATENT))
     qr = _mla_rows('q_rope', q_rope, (B, Sq, H, MLA_ROPE))
     for name, t, d in (('ckv', ckv, MLA_LATENT), ('k_rope', k_rope, MLA_ROPE)):
-        if tuple(t.shape) != (P, ps, d):
+        if t.shape != (P, ps, d):
             raise ValueError(f'{name} must be [{P}, {ps}, {d}], got {list(t.shape)}')
-        if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+        s0, s1, s2 = t.stride()
+        if s2 != 1 or (s0 | s1) & 7 or t.data_ptr() & 15:
             raise ValueError(f'{name} rows must be contiguous and 16-byte aligned')
     nb = block_table.shape[1]
-    out = torch.empty((B, Sq, H, MLA_LATENT), dtype=ql.dtype, device=ql.device)
-    wsb = int(N.load().lcq_mla_decode_workspace_bytes(B, Sq, H, nb * ps))
-    ws = torch.empty(wsb, dtype=torch.uint8, device=ql.device) if wsb else None
+    out = ql.new_empty((B, Sq, H, MLA_LATENT))
+    wsb = N.load().lcq_mla_decode_workspace_bytes(B, Sq, H, nb * ps)
+    ws = ql.new_empty(wsb, dtype=torch.uint8) if wsb else None
+    keep, st = _strides(ql, qr, ckv, k_rope)
     with N.on_device(ql):
-        N.call('lcq_mla_decode', N.ptr_strided(ql), _strides(ql, 3), N.ptr_strided(qr),
-               _strides(qr, 3), N.ptr_strided(ckv), _strides(ckv, 2), N.ptr_strided(k_rope),
-               _strides(k_rope, 2), P, ps, N.ptr(block_table), nb, N.ptr(kv_lens), N.dt(ql), B,
-               Sq, H, float(scale), N.ptr(out), N.ptr(ws), wsb, N.stream_of(ql))
+        N.call('lcq_mla_decode', ql.data_ptr(), st[0], qr.data_ptr(), st[1], ckv.data_ptr(),
+               st[2], k_rope.data_ptr(), st[3], P, ps, block_table.data_ptr(), nb,
+               kv_lens.data_ptr(), N.dt(ql), B, Sq, H, float(scale), out.data_ptr(),
+               None if ws is None else ws.data_ptr(), wsb, N.stream_of(ql))
     return out

@@ -39,7 +39,11 @@ def acts(g, *shape, dt, dev):
     (16, 128, 1024, 128), (17, 136, 1024, 1024), (31, 520, 4096, 128), (33, 64, 1056, 1056),
     (48, 1024, 256, 256), (64, 256, 640, 64), (65, 392, 2048, 128), (129, 640, 1152, 128),
     (200, 328, 512, 32), (257, 512, 768, 128), (511, 200, 512, 512), (1, 4096, 4096, 128),
-    (4, 2048, 7168, 128), (300, 1288, 2048, 64)])
+    (4, 2048, 7168, 128), (300, 1288, 2048, 64),
+    # a long k split over workgroups; the 128-row kernel: partial row and column tiles, every
+    # group kind, a last unit of 128 k that is cut, n whose AutoAWQ rows are not 16-byte aligned
+    (1, 64, 16384, 128), (7, 264, 12288, 64), (300, 8224, 384, 128), (129, 12320, 256, 256),
+    (1300, 2592, 352, 32), (700, 4160, 448, 64), (513, 4968, 256, 128), (900, 3360, 96, 96)])
 def test_linear(dev, layout, dt, m, n, k, group):
     from lightcompress_amd import ops
     g = torch.Generator().manual_seed(m * 7919 + n * 31 + k + group)
@@ -57,7 +61,7 @@ def test_linear_odd_columns_vllm(dev, m):
     """n of the vLLM layout is any number."""
     from lightcompress_amd import ops
     g = torch.Generator().manual_seed(m)
-    for n in (1, 15, 33, 131, 257):
+    for n in (1, 15, 33, 131, 257) + ((8201,) if m == 300 else ()):
         w = weight(g, 'vllm', n, 256, 64, dev)
         x = acts(g, m, 256, dt=torch.bfloat16, dev=dev)
         y, tol = R.linear(x, *w)
@@ -65,11 +69,11 @@ def test_linear_odd_columns_vllm(dev, m):
 
 
 @pytest.mark.parametrize('layout', LAYOUTS)
-@pytest.mark.parametrize('m', [3, 150])
-def test_linear_shapes_strides_bias(dev, layout, m):
+@pytest.mark.parametrize('m,n', [(3, 264), (150, 264), (150, 6240)])
+def test_linear_shapes_strides_bias(dev, layout, m, n):
     from lightcompress_amd import ops
     g = torch.Generator().manual_seed(5)
-    n, k = 264, 512
+    k = 512
     w = weight(g, layout, n, k, 128, dev)
     b = torch.randn(n, generator=g).to(torch.bfloat16).to(dev)
     big = acts(g, m, 2, k + 24, dt=torch.bfloat16, dev=dev)
@@ -85,11 +89,11 @@ def test_linear_shapes_strides_bias(dev, layout, m):
 
 
 @pytest.mark.parametrize('layout', LAYOUTS)
-@pytest.mark.parametrize('m', [4, 140])
-def test_linear_nan_and_inf_stay_in_their_row(dev, layout, m):
+@pytest.mark.parametrize('m,n', [(4, 256), (140, 256), (140, 12288)])
+def test_linear_nan_and_inf_stay_in_their_row(dev, layout, m, n):
     from lightcompress_amd import ops
     g = torch.Generator().manual_seed(8)
-    w = weight(g, layout, 256, 512, 64, dev)
+    w = weight(g, layout, n, 512, 64, dev)
     x = acts(g, m, 512, dt=torch.float16, dev=dev)
     x[1, 100], x[3, 511] = float('nan'), float('inf')
     got = ops.int4_linear(x, *w)
@@ -104,7 +108,8 @@ def test_linear_nan_and_inf_stay_in_their_row(dev, layout, m):
 @pytest.mark.parametrize('counts,n,k,group', [
     ([1], 128, 256, 128), ([0, 3, 0, 1, 0], 264, 512, 32), ([16, 17, 15, 0, 64], 136, 384, 128),
     ([0] * 70 + [5] + [0] * 90 + [33, 1], 128, 256, 64), ([300, 1, 129, 0, 40], 520, 1024, 128),
-    ([2] * 40, 72, 160, 160)])
+    ([2] * 40, 72, 160, 160), ([130, 0, 257], 288, 192, 64), ([64, 200], 104, 256, 128),
+    ([500], 416, 224, 32)])
 def test_grouped(dev, layout, dt, counts, n, k, group):
     """One and two weight sets, the SiLU product, gathered and sorted rows."""
     from lightcompress_amd import ops
@@ -133,13 +138,14 @@ def test_grouped(dev, layout, dt, counts, n, k, group):
             assert R.close(h[s], *R.silu_mul(*gu))
 
 
-def test_grouped_rows_outside_groups_and_bad_gather(dev):
+@pytest.mark.parametrize('rows', [40, 300])
+def test_grouped_rows_outside_groups_and_bad_gather(dev, rows):
     """Rows behind the last group stay as they were; a gather index out of range reads zeros;
     offsets outside the rows are clamped."""
     from lightcompress_amd import _native as N
     from lightcompress_amd import ops
     g = torch.Generator().manual_seed(3)
-    n, k, rows = 128, 256, 40
+    n, k = 128, 256
     ws = [weight(g, 'vllm', n, k, 128, dev) for _ in range(3)]
     tab = ops.int4_weight_table(ws, dev)
     x = acts(g, rows, k, dt=torch.bfloat16, dev=dev)
@@ -166,8 +172,8 @@ def test_other_stream_and_graph(dev):
     """On a side stream, and captured into a graph that is replayed on new inputs."""
     from lightcompress_amd import ops
     g = torch.Generator().manual_seed(4)
-    for m in (2, 90):
-        w = weight(g, 'autoawq', 256, 1024, 128, dev)
+    for m, n in ((2, 256), (90, 256), (200, 12288)):
+        w = weight(g, 'autoawq', n, 1024, 128, dev)
         x = acts(g, m, 1024, dt=torch.bfloat16, dev=dev)
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())

@@ -21,8 +21,9 @@ P = 1 << 20   # an address that is never touched
 
 
 def gemm(lib, dtype=N.BF16, ldx=256, m=4, k=256, x=P, qw=P, sc=P, qz=None, layout=0, group=128,
-         n=64, y=P, ldy=64):
-    rc = lib.lcq_int4_gemm(x, dtype, ldx, m, k, qw, sc, qz, layout, group, n, None, y, ldy, None)
+         n=64, y=P, ldy=64, ws=None, wsb=0):
+    rc = lib.lcq_int4_gemm(x, dtype, ldx, m, k, qw, sc, qz, layout, group, n, None, y, ldy, ws, wsb,
+                           None)
     return rc, lib.lcq_last_error().decode()
 
 
@@ -33,7 +34,9 @@ def gemm(lib, dtype=N.BF16, ldx=256, m=4, k=256, x=P, qw=P, sc=P, qz=None, layou
     (dict(layout=1), 'qzeros'), (dict(qz=P), 'qzeros'), (dict(x=P + 2), 'aligned'),
     (dict(qw=P + 4), 'aligned'), (dict(sc=P + 2), 'aligned'), (dict(ldx=252), 'stride'),
     (dict(ldx=248), 'stride'), (dict(ldy=63), 'stride'), (dict(x=None), 'null'),
-    (dict(m=-1), 'shape'), (dict(n=0), 'shape'), (dict(m=1 << 33), 'large')])
+    (dict(m=-1), 'shape'), (dict(n=0), 'shape'), (dict(m=1 << 33), 'large'),
+    (dict(n=1 << 26), 'large'), (dict(k=1 << 21, ldx=1 << 21), 'large'),
+    (dict(m=1, k=1 << 20, ldx=1 << 20), 'workspace')])
 def test_int4_gemm_refuses(lib, kw, msg):
     rc, err = gemm(lib, **kw)
     assert rc == -1 and msg in err, err
