@@ -189,15 +189,13 @@ struct I4Scales {
 #pragma unroll
     for (int f = 0; f < F; ++f) {
       const uint32_t gi = i4_group(a, (uint32_t)min(k0 + 128 / F * f, (int)a.k - 32));
-      const char* sp = reinterpret_cast<const char*>(sc);
       if constexpr (LAYOUT == LV) {
-        s[f][0] = *reinterpret_cast<const uint16_t*>(sp + (cols.so + 2 * gi));
+        s[f][0] = gload<uint16_t>(sc, cols.so + 2 * gi);
       } else {
-        const i4_v4u v = *reinterpret_cast<const i4_v4u*>(sp + (cols.so + gi * cols.lds));
+        const i4_v4u v = gload<i4_v4u>(sc, cols.so + gi * cols.lds);
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[f][j] = v[j];
-        z[f] = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(qz) +
-                                                  (cols.zo + gi * cols.ldw));
+        z[f] = gload<uint32_t>(qz, cols.zo + gi * cols.ldw);
       }
     }
   }
@@ -291,6 +289,7 @@ __global__ __launch_bounds__(64 * W) void k_int4_few(I4Args a) {
 #pragma unroll
     for (int t = 0; t < T; ++t) acc[i][t] = zero;
   const i4_v4u ones = {i4_ones<DT>, i4_ones<DT>, i4_ones<DT>, i4_ones<DT>};
+  const I4Const<DT> kc;
 
   const int nb = (int)((a.k + 127) / 128);
   const int sp = a.row_off ? 0 : blockIdx.z;
@@ -313,8 +312,7 @@ __global__ __launch_bounds__(64 * W) void k_int4_few(I4Args a) {
       for (int s = 0; s < SETS; ++s)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-          wv[s][t] = *reinterpret_cast<const i4_v4u*>(reinterpret_cast<const char*>(qw[s]) +
-                                                      (cols.wo[t] + kw));
+          wv[s][t] = gload<i4_v4u>(qw[s], cols.wo[t] + kw);
     }
 #pragma unroll
     for (int s = 0; s < SETS; ++s) scl[slot][s].load(a, cols, sc[s], qz[s], k0);
@@ -324,12 +322,11 @@ __global__ __launch_bounds__(64 * W) void k_int4_few(I4Args a) {
         const uint16_t* p = xr[i] + (k0 + (LAYOUT == LA ? 8 * q : 32 * q));
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          xf[slot][i][j] = *reinterpret_cast<const i4_v4u*>(p + (LAYOUT == LA ? 32 * j : 8 * j));
+          xf[slot][i][j] = gload_at<i4_v4u>(p + (LAYOUT == LA ? 32 * j : 8 * j));
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)  // steps past k are not computed
-          xf[slot][i][j] =
-              *reinterpret_cast<const i4_v4u*>(xr[i] + (min(k0 + 32 * j, (int)a.k - 32) + 8 * q));
+          xf[slot][i][j] = gload_at<i4_v4u>(xr[i] + (min(k0 + 32 * j, (int)a.k - 32) + 8 * q));
       }
     }
   };
@@ -375,8 +372,8 @@ __global__ __launch_bounds__(64 * W) void k_int4_few(I4Args a) {
           }
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            const i4_v4u bf = LAYOUT == LV ? i4_word<DT>(wv[s][LAYOUT == LV ? t : 0][j])
-                                           : i4_nibble<DT>(pk, t);
+            const i4_v4u bf = LAYOUT == LV ? i4_word<DT>(wv[s][LAYOUT == LV ? t : 0][j], kc)
+                                           : i4_nibble<DT>(pk, t, kc);
 #pragma unroll
             for (int i = 0; i < MT; ++i)
               g[i][s * NT + t] = i4_mfma<DT>(xf[slot][i][j], bf, g[i][s * NT + t]);
@@ -531,7 +528,7 @@ __global__ __launch_bounds__(512, 2) void k_int4_tile(I4Args a) {
   auto x_load = [&](int u) {  // vLLM: to registers
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      xg[i] = *reinterpret_cast<const i4_v4u*>(xr[i] + min(128 * u + 8 * c, k - 8));
+      xg[i] = gload_at<i4_v4u>(xr[i] + min(128 * u + 8 * c, k - 8));
   };
   auto x_store = [&](uint32_t buf) {
 #pragma unroll
@@ -592,19 +589,18 @@ __global__ __launch_bounds__(512, 2) void k_int4_tile(I4Args a) {
       const uint32_t kw = (uint32_t)min(k0 + 32 * q, k - 32) / 2;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
-        wv[t] = *reinterpret_cast<const i4_v4u*>(
-            reinterpret_cast<const char*>(qw[SETS == 2 ? t >> 1 : 0]) + (wo[t] + kw));
+        wv[t] = gload<i4_v4u>(qw[SETS == 2 ? t >> 1 : 0], wo[t] + kw);
     }
 #pragma unroll
     for (int f = 0; f < F; ++f) {
       const uint32_t gi = i4_group(a, (uint32_t)min(k0 + 128 / F * f, k - 32));
       if constexpr (LAYOUT == LV) {
-        sv4[f][0] = *reinterpret_cast<const uint16_t*>(sp + (so + 2 * gi));
+        sv4[f][0] = gload<uint16_t>(sp, so + 2 * gi);
       } else {
-        const i4_v4u v = *reinterpret_cast<const i4_v4u*>(sp + (so + gi * lds_s));
+        const i4_v4u v = gload<i4_v4u>(sp, so + gi * lds_s);
 #pragma unroll
         for (int j = 0; j < 4; ++j) sv4[f][j] = v[j];
-        zv1[f] = *reinterpret_cast<const uint32_t*>(zp + (zo + gi * ldw));
+        zv1[f] = gload<uint32_t>(zp, zo + gi * ldw);
       }
     }
   };
@@ -615,6 +611,7 @@ __global__ __launch_bounds__(512, 2) void k_int4_tile(I4Args a) {
   };
   const i4_v4f zero = {0.f, 0.f, 0.f, 0.f};
   const i4_v4u ones = {i4_ones<DT>, i4_ones<DT>, i4_ones<DT>, i4_ones<DT>};
+  const I4Const<DT> kc;
   auto x_sums = [&](int u, uint32_t buf) {  // of row tile 4 mh + nw, to the unit's sum buffer
 #pragma unroll
     for (int f = 0; f < F; ++f) {
@@ -721,8 +718,8 @@ __global__ __launch_bounds__(512, 2) void k_int4_tile(I4Args a) {
         for (int i = 0; i < 4; ++i) g[i] = LAYOUT == LV ? xs[i] : -z * xs[i];
 #pragma unroll
         for (int j = 0; j < 4 / F; ++j) {
-          const i4_v4u bf = LAYOUT == LV ? i4_word<DT>(wc4[LAYOUT == LV ? t : 0][4 / F * f + j])
-                                         : i4_nibble<DT>(pk[LAYOUT == LA ? j : 0], t);
+          const i4_v4u bf = LAYOUT == LV ? i4_word<DT>(wc4[LAYOUT == LV ? t : 0][4 / F * f + j], kc)
+                                         : i4_nibble<DT>(pk[LAYOUT == LA ? j : 0], t, kc);
 #pragma unroll
           for (int i = 0; i < 4; ++i) g[i] = i4_mfma<DT>(xf[i][4 / F * f + j], bf, g[i]);
         }

@@ -33,31 +33,57 @@ __device__ __forceinline__ i4_v4f i4_mfma(i4_v4u a, i4_v4u b, i4_v4f c) {
 template <int DT>
 constexpr uint32_t i4_ones = DT == LCQ_BF16 ? 0x3f803f80u : 0x3c003c00u;
 
+// The mask and the base of a pair of codes, in a vector and a scalar register: as literals the and
+// and the or would be two instructions (one instruction takes no literal and one scalar)
+template <int DT>
+struct I4Const {
+  uint32_t mask = DT == LCQ_BF16 ? 0x00780078u : 0x03c003c0u;
+  uint32_t base = DT == LCQ_BF16 ? 0x41804180u : 0x4c004c00u;
+  __device__ __forceinline__ I4Const() {
+    asm volatile("" : "+v"(mask));
+    asm volatile("" : "+s"(base));
+  }
+};
+
 // nibbles P and P + 4 of w as 16 + code in the low and high half (P = 0..3)
 template <int DT, int P>
-__device__ __forceinline__ uint32_t i4_pair(uint32_t w) {
-  constexpr int at = DT == LCQ_BF16 ? 3 : 6;  // target bit of the code
-  constexpr uint32_t mask = DT == LCQ_BF16 ? 0x00780078u : 0x03c003c0u;
-  constexpr uint32_t base = DT == LCQ_BF16 ? 0x41804180u : 0x4c004c00u;
-  constexpr int sh = at - 4 * P;
-  if constexpr (sh >= 0) return ((w << sh) & mask) | base;
-  else return ((w >> -sh) & mask) | base;
+__device__ __forceinline__ uint32_t i4_pair(uint32_t w, const I4Const<DT>& k) {
+  constexpr int sh = (DT == LCQ_BF16 ? 3 : 6) - 4 * P;  // to the top of the mantissa
+  if constexpr (sh >= 0) return ((w << sh) & k.mask) | k.base;
+  else return ((w >> -sh) & k.mask) | k.base;
 }
 
 // one word of 8 codes along k as a B fragment, elements in the order 0 4 1 5 2 6 3 7
 template <int DT>
-__device__ __forceinline__ i4_v4u i4_word(uint32_t w) {
-  return i4_v4u{i4_pair<DT, 0>(w), i4_pair<DT, 1>(w), i4_pair<DT, 2>(w), i4_pair<DT, 3>(w)};
+__device__ __forceinline__ i4_v4u i4_word(uint32_t w, const I4Const<DT>& k) {
+  return i4_v4u{i4_pair<DT, 0>(w, k), i4_pair<DT, 1>(w, k), i4_pair<DT, 2>(w, k),
+                i4_pair<DT, 3>(w, k)};
 }
 
 // nibble t of every half of four packed pairs
 template <int DT>
-__device__ __forceinline__ i4_v4u i4_nibble(i4_v4u v, int t) {
+__device__ __forceinline__ i4_v4u i4_nibble(i4_v4u v, int t, const I4Const<DT>& k) {
   auto f = [&](uint32_t w) {
-    return t == 0 ? i4_pair<DT, 0>(w) : t == 1 ? i4_pair<DT, 1>(w) : t == 2 ? i4_pair<DT, 2>(w)
-                                                                           : i4_pair<DT, 3>(w);
+    return t == 0   ? i4_pair<DT, 0>(w, k)
+           : t == 1 ? i4_pair<DT, 1>(w, k)
+           : t == 2 ? i4_pair<DT, 2>(w, k)
+                    : i4_pair<DT, 3>(w, k);
   };
   return i4_v4u{f(v.x), f(v.y), f(v.z), f(v.w)};
+}
+
+// load from a wave-uniform base + a lane's 32-bit offset, as a global (not a flat) load: flat loads
+// count against the LDS waits too
+template <typename T>
+__device__ __forceinline__ T gload(const void* base, uint32_t off) {
+  typedef const __attribute__((address_space(1))) char gchar;
+  typedef const __attribute__((address_space(1))) T gT;
+  return *reinterpret_cast<gT*>(reinterpret_cast<gchar*>(reinterpret_cast<uint64_t>(base)) + off);
+}
+template <typename T>
+__device__ __forceinline__ T gload_at(const void* p) {
+  typedef const __attribute__((address_space(1))) T gT;
+  return *reinterpret_cast<gT*>(reinterpret_cast<uint64_t>(p));
 }
 
 // 8 consecutive x values as an A fragment in that order
