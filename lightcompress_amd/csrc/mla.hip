@@ -37,12 +37,19 @@ __device__ __forceinline__ const uint16_t* uni(const uint16_t* p) {
   return reinterpret_cast<const uint16_t*>(((uint64_t)hi << 32) | lo);
 }
 
+__device__ __forceinline__ int64_t uni(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
 // ---------------------------------------------------------------------------------------
 // Expanded form
 // ---------------------------------------------------------------------------------------
 constexpr int FQT = 128;  // query rows per workgroup (4 waves of 32)
 constexpr int FKT = 64;   // keys per tile
 constexpr int F_STAGE = FKT * (DN + DR + DV) * 2;  // 40 KB
+constexpr int F_AHEAD = 6;                         // LDS fragments read ahead of their product
 
 struct MlaFwdArgs {
   const uint16_t *qn, *qr, *kn, *kr, *v;
@@ -54,30 +61,37 @@ struct MlaFwdArgs {
   float sl2;                // scale * log2(e)
 };
 
-// One 64-key tile of the three images by LDS-DMA: 10 instructions per wave. The base moves with the
-// tile (64-bit), so only a tile's own span has to fit 32 bits. Keys past `last` re-read it: what
-// lies behind a sequence is never loaded.
-__device__ __forceinline__ void fwd_stage(uint32_t st, const uint16_t* kn, const uint16_t* kr,
-                                          const uint16_t* v, const MlaFwdArgs& a, int k0, int last,
-                                          int w, int lane) {
-  const uint16_t *bn = uni(kn + k0 * a.kns), *bv = uni(v + k0 * a.vs), *br = uni(kr + k0 * a.krs);
-  const int lim = last - k0;
+// The three images of one 64-key tile by LDS-DMA, 10 instructions per wave. The base moves with the
+// tile (64-bit), so only a tile's own span has to fit 32 bits; a lane's offsets are formed once
+// (`lim` 63) and again for a last tile, whose keys past `lim` re-read it: what lies behind a
+// sequence is never loaded.
+struct FwdStage {
+  uint32_t kn[4], v[4], kr[2];
+  __device__ __forceinline__ void init(const MlaFwdArgs& a, int lim, int w, int lane) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int row = 4 * (4 * w + j) + (lane >> 4);
-    const int ch = (lane & 15) ^ swz16(row);
-    const uint32_t key = min(row, lim);
-    dma16(st + 1024 * (4 * w + j), bn, key * (uint32_t)a.kns * 2 + ch * 16);
-    dma16(st + 16384 + 1024 * (4 * w + j), bv, key * (uint32_t)a.vs * 2 + ch * 16);
-  }
+    for (int j = 0; j < 4; ++j) {
+      const int row = 4 * (4 * w + j) + (lane >> 4);
+      const uint32_t ch = 16 * ((lane & 15) ^ swz16(row)), key = min(row, lim);
+      kn[j] = key * (uint32_t)a.kns * 2 + ch;
+      v[j] = key * (uint32_t)a.vs * 2 + ch;
+    }
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int row = 8 * (2 * w + j) + (lane >> 3);
-    const int ch = (lane & 7) ^ ((row >> 1) & 7);
-    const uint32_t key = min(row, lim);
-    dma16(st + 32768 + 1024 * (2 * w + j), br, key * (uint32_t)a.krs * 2 + ch * 16);
+    for (int j = 0; j < 2; ++j) {
+      const int row = 8 * (2 * w + j) + (lane >> 3);
+      kr[j] = (uint32_t)min(row, lim) * (uint32_t)a.krs * 2 + 16 * ((lane & 7) ^ ((row >> 1) & 7));
+    }
   }
-}
+  __device__ __forceinline__ void issue(uint32_t st, const uint16_t* pn, const uint16_t* pr,
+                                        const uint16_t* pv, int w) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      dma16(st + 1024 * (4 * w + j), pn, kn[j]);
+      dma16(st + 16384 + 1024 * (4 * w + j), pv, v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) dma16(st + 32768 + 1024 * (2 * w + j), pr, kr[j]);
+  }
+};
 
 template <int DT>
 __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
@@ -109,10 +123,17 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
   }
   const uint16_t* qnp = a.qn + b * a.qnb + hq * a.qnh;
   const uint16_t* qrp = a.qr + b * a.qrb + hq * a.qrh;
-  const uint16_t* knp = a.kn + b * a.knb + hq * a.knh;
-  const uint16_t* krp = a.kr + b * a.krb;
-  const uint16_t* vp = a.v + b * a.vb + hq * a.vh;
-  fwd_stage(lds0, knp, krp, vp, a, 0, klen - 1, w, lane);
+  const uint16_t* knp = uni(a.kn + b * a.knb + hq * a.knh);
+  const uint16_t* krp = uni(a.kr + b * a.krb);
+  const uint16_t* vp = uni(a.v + b * a.vb + hq * a.vh);
+  FwdStage fs;
+  fs.init(a, min(FKT - 1, klen - 1), w, lane);
+  auto stage = [&](int k0, int buf) {  // called for tile after tile
+    if (k0 > 0 && klen - 1 - k0 < FKT - 1) fs.init(a, klen - 1 - k0, w, lane);
+    fs.issue(lds0 + buf * F_STAGE, uni(knp + k0 * a.kns), uni(krp + k0 * a.krs),
+             uni(vp + k0 * a.vs), w);
+  };
+  stage(0, 0);
 
   const int qrow = q0 + 32 * w + c;  // this lane's query row (both halves)
   // Q^T as the B operand of mfma(K, Q^T): lane holds Q[qrow][16 kk + 8 h + j]
@@ -143,28 +164,35 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
   int it = 0;
   for (int k0 = 0; k0 < kend; k0 += FKT, ++it) {
     const uint32_t cur = lds0 + (it & 1) * F_STAGE;
-    // every wave is done with the stage the next tile overwrites
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    // this wave's part of the tile has arrived; behind the barrier every wave's has, and every
+    // wave is done with the tile before, whose stage is filled next
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    if (k0 + FKT < kend) {
-      fwd_stage(lds0 + ((it & 1) ^ 1) * F_STAGE, knp, krp, vp, a, k0 + FKT, klen - 1, w, lane);
-      asm volatile("s_waitcnt vmcnt(10)" ::: "memory");  // this tile's loads, not the next's
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    __builtin_amdgcn_s_barrier();  // this tile is in LDS for every wave
-    // S^T tiles t: register r holds key k0 + 32 t + (r & 3) + 8 (r >> 2) + 4 h of the lane's row
+    if (k0 + FKT < kend) stage(k0 + FKT, (it & 1) ^ 1);
+
+    // S^T tiles t: register r holds key k0 + 32 t + (r & 3) + 8 (r >> 2) + 4 h of the lane's row.
+    // The two tiles in turn, so that a product does not wait for the one before it; K fragments
+    // are read F_AHEAD products ahead (the scheduling barriers keep the compiler to that order:
+    // left alone it waits for each read right before its product)
     v16f_t s[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.f;
+    {
+      const uint32_t kb = cur + ka, rp = cur + ra;
+      auto kfrag = [&](int f) {  // product f: k-step f / 2 of tile f & 1
+        const int kk = f >> 1, t = f & 1;
+        return kk < 8 ? lds_read16((kb ^ (32 * kk)) + 8192 * t)
+                      : lds_read16((rp ^ (32 * (kk - 8))) + 4096 * t);
+      };
+      v8s_t kf[F_AHEAD];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+      for (int f = 0; f < F_AHEAD; ++f) kf[f] = kfrag(f);
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk)
-        s[t] = mfma32<DT>(lds_read16(((cur + ka) ^ (32 * kk)) + 8192 * t), qf[kk], s[t]);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        s[t] = mfma32<DT>(lds_read16(((cur + ra) ^ (32 * kk)) + 4096 * t), qf[8 + kk], s[t]);
+      for (int f = 0; f < 24; ++f) {
+        s[f & 1] = mfma32<DT>(kf[f % F_AHEAD], qf[f >> 1], s[f & 1]);
+        if (f + F_AHEAD < 24) kf[f % F_AHEAD] = kfrag(f + F_AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     if (k0 + FKT - 1 > wmin) {  // wave-uniform: some key is hidden from some row
       const int lim = pos - k0 - 4 * h;
@@ -180,9 +208,19 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
     mx = fmaxf(mx, other_half(mx, h)) * a.sl2;  // sl2 > 0: max commutes with the scale
-    const float mn = fmaxf(m, mx);
-    const float alpha = (mn == -INFINITY) ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-    const float msub = (mn == -INFINITY) ? 0.f : mn;
+    // the output is rescaled only when a row's maximum has grown by more than 2^8 since it last
+    // was: weights stay below 2^8, in range of fp16
+    if (__any(mx > m + 8.f)) {
+      const float mn = mx > m + 8.f ? mx : m;
+      const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= alpha;
+      m = mn;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+    }
+    const float msub = m == -INFINITY ? 0.f : m;
     float rs = 0.f;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -192,35 +230,34 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
         s[t][r] = p;
         rs += p;
       }
-    rs += other_half(rs, h);
-    l = l * alpha + rs;
-    m = mn;
-    if (alpha != 1.f) {
+    l += rs + other_half(rs, h);
+    // O^T += V^T P^T; k-step ts = (t, s2): score registers 8 s2 .. 8 s2 + 7 of tile t, V^T fragments
+    // by transposed reads of the same keys' rows
+    v8s_t pf[4];
 #pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
+    for (int ts = 0; ts < 4; ++ts) {
+      uint32_t* pw = reinterpret_cast<uint32_t*>(&pf[ts]);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+      for (int j = 0; j < 4; ++j)
+        pw[j] = pack_dt<DT>(s[ts >> 1][8 * (ts & 1) + 2 * j], s[ts >> 1][8 * (ts & 1) + 2 * j + 1]);
     }
-    // O^T += V^T P^T; k-step (t, s2): score registers 8 s2 .. 8 s2 + 7 of tile t, V^T fragments by
-    // transposed reads of the same keys' rows
+    {
+      const uint32_t vb = cur + va;
+      auto vfrag = [&](int f) {  // product f: k-step f / 4, dims 32 (f & 3) ..
+        const uint32_t at = (vb ^ (64 * (f & 3))) + 4096 * (f >> 2);
+        const v4s_t lo = lds_read_tr(at), hi = lds_read_tr((at ^ 32) + 2048);
+        return (v8s_t){lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      };
+      v8s_t vf[F_AHEAD];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int f = 0; f < F_AHEAD; ++f) vf[f] = vfrag(f);
 #pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) {
-        v8s_t pf;
-        uint32_t* pw = reinterpret_cast<uint32_t*>(&pf);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          pw[j] = pack_dt<DT>(s[t][8 * s2 + 2 * j], s[t][8 * s2 + 2 * j + 1]);
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt) {
-          const uint32_t at = (cur + va) ^ (64 * dt);
-          const v4s_t lo = lds_read_tr(at + 256 * (32 * t + 16 * s2));
-          const v4s_t hi = lds_read_tr((at ^ 32) + 256 * (32 * t + 16 * s2 + 8));
-          const v8s_t vf = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-          o[dt] = mfma32<DT>(vf, pf, o[dt]);
-        }
+      for (int f = 0; f < 16; ++f) {
+        o[f & 3] = mfma32<DT>(vf[f % F_AHEAD], pf[f >> 2], o[f & 3]);
+        if (f + F_AHEAD < 16) vf[f % F_AHEAD] = vfrag(f + F_AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
       }
+    }
   }
   __syncthreads();
   // a row that saw no key has l = 0: zeros (a NaN l stays one)
@@ -253,11 +290,22 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
 // ---------------------------------------------------------------------------------------
 constexpr int DKT = 32;                          // keys per tile
 constexpr int D_STAGE = DKT * (DL + DR) * 2;     // 36 KB: latent rows of 1 KB, rotary rows of 128 B
-constexpr int D_TAB = 2048;                      // keys whose page numbers are held in LDS at a time
+constexpr int D_RING = 8;                        // tiles whose key addresses are held in LDS
+// tiles whose page numbers are held in LDS at a time: what the stages leave of 160 / 80 KB
+constexpr int dec_tab(int nst) { return nst == 4 ? 64 : 16; }
 constexpr int D_ROWS = 16;                       // query rows (token x head) per wave
 constexpr int D_PART = D_ROWS * DL;              // floats of one row block's partial output
+constexpr int D_MIN = 2;                         // least tiles of a workgroup
+constexpr int D_AHEAD = 4;                       // LDS fragments read ahead of their product
 
 typedef float v4f_t __attribute__((ext_vector_type(4)));
+
+// XOR of the 16 low chunks of a latent row: 16 rows differ (the row reads), and of the rows 4 q + i
+// that 32 lanes read transposed, those of q = 0, 1 (2, 3) differ in chunk bit 1, which those reads
+// leave free (with swz16, whose rows 4 apart differ in bit 0, every transposed read met a conflict)
+__device__ __forceinline__ int dec_swz(int row) {
+  return ((row & 3) << 2) | ((row >> 1) & 2) | ((row >> 3) & 1);
+}
 
 template <int DT>
 __device__ __forceinline__ v4f_t mfma16(v8s_t a, v8s_t b, v4f_t c) {
@@ -291,12 +339,63 @@ struct MlaDecArgs {
   const int32_t* table;     // [B, nb]
   const int32_t* lens;      // [B]
   uint16_t* out;            // [B, Sq, H, 512]
-  float* part;              // [splits][B][nrb][D_PART]
-  float* ml;                // [splits][B][nrb][16][2]
+  float* part;              // [2 * wgs][RB][D_PART]
+  float* ml;                // [2 * wgs][RB][16][2]
   int64_t P;
-  int B, Sq, H, ps, nb, nrb, chunk, nsplit;
+  int B, Sq, H, ps, nb, nrb, ny, wgs;  // nrb row blocks, ny = ceil(nrb / RB) of a workgroup
   float sl2;
 };
+
+// ---- how the work is divided -----------------------------------------------------------
+// A sequence b takes n_b = max(1, ceil(len / 32)) key tiles, once for each of its ny groups of RB row
+// blocks. The tiles of all (b, group) stand in one line, b major, and the line is cut into wgs
+// equal ranges (fewer where a range would fall below D_MIN tiles), one workgroup each: whatever
+// the lengths, the workgroups do the same work. A (b, group) inside one range is finished by its
+// workgroup; one that a cut divides leaves partial outputs in its workgroups' slots, 2 i for the
+// segment that workgroup i begins with, 2 i + 1 for another one, and k_mla_join adds them in order.
+__device__ __forceinline__ int dec_len(const MlaDecArgs& a, int b) {
+  return (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.nb * a.ps);
+}
+__device__ __forceinline__ int dec_tiles(const MlaDecArgs& a, int b) {
+  return max(1, (dec_len(a, b) + DKT - 1) / DKT);
+}
+// total tiles over all (b, group); with find, also the sequence that holds tile `at` and the first
+// tile of that sequence
+__device__ __forceinline__ int dec_total(const MlaDecArgs& a) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int b = lane; b < a.B; b += 64) n += dec_tiles(a, b);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
+  return __builtin_amdgcn_readfirstlane(n) * a.ny;
+}
+// the sequence that holds tile `at`, and its first tile
+__device__ __forceinline__ int dec_find(const MlaDecArgs& a, int at, int& first) {
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + lane;
+    const int t = b < a.B ? dec_tiles(a, b) * a.ny : 0;
+    int inc = t;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(inc, d);
+      if (lane >= d) inc += o;
+    }
+    const int total = __builtin_amdgcn_readfirstlane(__shfl(inc, 63));
+    if (at < base + total) {
+      const int l = __builtin_ctzll(__ballot(at < base + inc));
+      first = __builtin_amdgcn_readfirstlane(base + __shfl(inc - t, l));
+      return __builtin_amdgcn_readfirstlane(b0 + l);
+    }
+    base += total;
+  }
+  return a.B;
+}
+// tiles of a range
+__device__ __forceinline__ int dec_step(const MlaDecArgs& a, int total) {
+  return max(D_MIN, (total + a.wgs - 1) / a.wgs);
+}
 
 // One wave per 16 query rows, RB waves per workgroup sharing the key tiles. Scores are held
 // transposed (mfma(K, Q^T): a lane has 8 keys of one row), so they turn into the B operand of
@@ -305,207 +404,288 @@ struct MlaDecArgs {
 template <int DT, int RB, int NST>
 __global__ void __launch_bounds__(64 * RB, 2) k_mla_dec(MlaDecArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char mla_lds[];
-  int32_t* tab = reinterpret_cast<int32_t*>(mla_lds + NST * D_STAGE);
+  // addresses of the keys of D_RING tiles: [tile][32] {latent row, rotary row}, and their masks
+  typedef uint64_t addr_t[DKT][2];
+  addr_t* addrs = reinterpret_cast<addr_t*>(mla_lds + NST * D_STAGE);
+  uint32_t* mask_of = reinterpret_cast<uint32_t*>(mla_lds + NST * D_STAGE +
+                                                  D_RING * sizeof(addr_t));
+  int32_t* tab = reinterpret_cast<int32_t*>(mask_of + D_RING);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, q = lane >> 4;
-  const int sp = blockIdx.x, b = blockIdx.z;
-  const int rb = blockIdx.y * RB + w;  // this wave's row block
   const int rows = a.Sq * a.H;
-  const int len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.nb * a.ps);
-  const int kbeg = sp * a.chunk, kend = min(len, kbeg + a.chunk);
-  const int row = D_ROWS * rb + c;
-  const int qi = row / a.H, qh = row - qi * a.H;
-  const bool live = row < rows;
   const uint32_t lds0 = lds_addr(mla_lds);
-
-  v8s_t qf[18];  // Q^T as the B operand: Q[row][32 kk + 8 q + j]
-#pragma unroll
-  for (int kk = 0; kk < 18; ++kk) {
-    qf[kk] = (v8s_t){0, 0, 0, 0, 0, 0, 0, 0};
-    if (live)
-      qf[kk] = *reinterpret_cast<const v8s_t*>(
-          kk < 16 ? a.ql + b * a.qlb + qi * a.qls + qh * a.qlh + 32 * kk + 8 * q
-                  : a.qr + b * a.qrb + qi * a.qrs + qh * a.qrh + 32 * (kk - 16) + 8 * q);
+  const int total = dec_total(a), step = dec_step(a, total);
+  // neighbouring ranges (a sequence's) on one XCD
+  int wg;
+  {
+    const int p = (int)blockIdx.x, nwg = (int)gridDim.x;
+    const int xcd = p & 7, q8 = nwg >> 3, r8 = nwg & 7;
+    wg = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (p >> 3);
   }
-  const int pos = len - a.Sq + qi;  // last key this lane's row sees
-  float m = -INFINITY, l = 0.f;
-  const v4f_t zero = {0.f, 0.f, 0.f, 0.f};
-  v4f_t o[32];
-#pragma unroll
-  for (int dt = 0; dt < 32; ++dt) o[dt] = zero;
-
+  int at = wg * step;
+  if (at >= total) return;
+  const int end = min(total, at + step), begin = at;
   // LDS offsets in a stage; a constant XOR walks the swizzled chunks of a row
   const int q4 = c >> 2, pp = c & 3;
-  const uint32_t ka = 1024 * c + 16 * (q ^ swz16(c));                      // chunk 4 kk + q
+  const uint32_t ka = 1024 * c + 16 * (q ^ dec_swz(c));                    // chunk 4 kk + q
   const uint32_t ra = DKT * 1024 + 128 * c + 16 * (q ^ ((c >> 1) & 7));     // rotary chunk
-  const uint32_t va = 1024 * (4 * q + q4) + 16 * ((pp >> 1) ^ (q4 << 2 | q)) + 8 * (pp & 1);
+  const uint32_t va = 1024 * (4 * q + q4) + 16 * ((pp >> 1) ^ dec_swz(4 * q + q4)) + 8 * (pp & 1);
+  const v4f_t zero = {0.f, 0.f, 0.f, 0.f};
 
-  // Stage the tile of keys kb .. kb + 31; returns the mask of its keys that exist. A key past the
-  // end or on a page outside the pool is loaded from the tile's first existing key (or the pool's
-  // first row): nothing behind a sequence is read.
-  auto stage = [&](uint32_t st, int kb, int p0) -> uint32_t {
-    const int key = kb + (lane & 31);
-    const int pg = key / a.ps, slot = key - pg * a.ps;
-    const int page = key < kend ? tab[pg - p0] : -1;
-    const bool ok = page >= 0 && page < a.P;
-    const uint32_t mask = (uint32_t)__ballot(ok);
-    const int src = mask ? __builtin_ctz(mask) : 0;
-    uint64_t cb = reinterpret_cast<uint64_t>(a.ckv), rbs = reinterpret_cast<uint64_t>(a.kr);
-    if (ok) {
-      cb += 2 * (page * a.cp + slot * a.cs);
-      rbs += 2 * (page * a.rp + slot * a.rs);
-    }
-    const uint64_t cb0 = __shfl(cb, src), rb0 = __shfl(rbs, src);
-    if (!ok) { cb = cb0; rbs = rb0; }
+  int first;
+  int b = dec_find(a, at, first);
+  while (at < end) {
+    const int len = __builtin_amdgcn_readfirstlane(dec_len(a, b));
+    const int nt = max(1, (len + DKT - 1) / DKT);
+    const int y = __builtin_amdgcn_readfirstlane((at - first) / nt);
+    const int t0 = at - first - y * nt, t1 = min(nt, t0 + (end - at));
+    const int rb = y * RB + w;  // this wave's row block
+
+    int p0 = 0;  // page that tab begins with
+    // Addresses of tile t's keys, by 32 lanes of one wave (page numbers from LDS: a load from memory
+    // here would wait for every tile in flight). A key past the length or on a page
+    // outside the pool takes the tile's first existing key (or the pool's first row): nothing
+    // behind a sequence is read.
+    auto locate = [&](int t) {
+      const int key = DKT * t + (lane & 31);
+      const int pg = key / a.ps, slot = key - pg * a.ps;
+      const int page = key < len ? tab[pg - p0] : -1;
+      const bool ok = page >= 0 && page < a.P;
+      const uint32_t mask = (uint32_t)__ballot(ok);
+      const int src = mask ? __builtin_ctz(mask) : 0;
+      uint64_t cb = reinterpret_cast<uint64_t>(a.ckv), rbs = reinterpret_cast<uint64_t>(a.kr);
+      if (ok) {
+        cb += 2 * (page * a.cp + slot * a.cs);
+        rbs += 2 * (page * a.rp + slot * a.rs);
+      }
+      const uint64_t cb0 = __shfl(cb, src), rb0 = __shfl(rbs, src);
+      if (!ok) { cb = cb0; rbs = rb0; }
+      if (lane < 32) {
+        addrs[t % D_RING][lane][0] = cb;
+        addrs[t % D_RING][lane][1] = rbs;
+      }
+      if (lane == 0) mask_of[t % D_RING] = mask;
+    };
+    auto stage = [&](int t) {  // tile t's rows: DKT / RB + (w < 4) LDS-DMA instructions a wave
+      const uint32_t st = lds0 + (t % NST) * D_STAGE;
+      const addr_t& ad = addrs[t % D_RING];
+#pragma unroll 4
+      for (int j = 0; j < DKT / RB; ++j) {
+        const int r = w * (DKT / RB) + j;
+        dma16_at(st + 1024 * r, ad[r][0] + (lane ^ dec_swz(r)) * 16);
+      }
+#pragma unroll 1
+      for (int g8 = w; g8 < DKT / 8; g8 += RB) {  // rotary rows, 8 keys an instruction
+        const int r = 8 * g8 + (lane >> 3);
+        dma16_at(st + DKT * 1024 + 1024 * g8, ad[r][1] + ((lane & 7) ^ ((r >> 1) & 7)) * 16);
+      }
+    };
+
+    // a lane past the last row computes it again and stores nothing
+    const int qrow = min(D_ROWS * rb + c, rows - 1), qi = qrow / a.H, qh = qrow - qi * a.H;
+    v8s_t qf[18];  // Q^T as the B operand: Q[row][32 kk + 8 q + j]
+    {
+      const uint16_t* ql = a.ql + b * a.qlb + qi * a.qls + qh * a.qlh + 8 * q;
+      const uint16_t* qr = a.qr + b * a.qrb + qi * a.qrs + qh * a.qrh + 8 * q;
 #pragma unroll
-    for (int j = 0; j < DKT / RB; ++j) {
-      const int r = w * (DKT / RB) + j;
-      const uint64_t row = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(cb >> 32), r)
-                            << 32) |
-                           (uint32_t)__builtin_amdgcn_readlane((uint32_t)cb, r);
-      dma16(st + 1024 * r, reinterpret_cast<const void*>(row), (lane ^ swz16(r)) * 16);
+      for (int kk = 0; kk < 18; ++kk)
+        qf[kk] = *reinterpret_cast<const v8s_t*>(kk < 16 ? ql + 32 * kk : qr + 32 * (kk - 16));
     }
-    // rotary rows, 8 keys an instruction
-    for (int g8 = w; g8 < DKT / 8; g8 += RB) {
-      const int r = 8 * g8 + (lane >> 3);
-      dma16_at(st + DKT * 1024 + 1024 * g8,
-               __shfl(rbs, r) + ((lane & 7) ^ ((r >> 1) & 7)) * 16);
-    }
-    return mask;
-  };
+    const int pos = len - a.Sq + qi;  // last key this lane's row sees
+    float m = -INFINITY, l = 0.f;
+    v4f_t o[32];
+#pragma unroll
+    for (int dt = 0; dt < 32; ++dt) o[dt] = zero;
 
-  for (int kt = kbeg; kt < kend; kt += D_TAB) {
-    const int ke = min(kend, kt + D_TAB);
-    const int p0 = kt / a.ps, p1 = (ke - 1) / a.ps;
+    for (int tb = t0; tb < t1; tb += dec_tab(NST)) {
+    const int te = min(t1, tb + dec_tab(NST));
+    p0 = DKT * tb / a.ps;
+    const int np = (min(len, DKT * te) - 1) / a.ps - p0 + 1;  // 0 for an empty sequence
+    __syncthreads();  // the tiles before are done with the stages and the addresses
+    for (int i = tid; i < np; i += 64 * RB) tab[i] = a.table[(int64_t)b * a.nb + p0 + i];
     __syncthreads();
-    for (int i = tid; i <= p1 - p0; i += 64 * RB) tab[i] = a.table[(int64_t)b * a.nb + p0 + i];
+    for (int i = w; i < NST + 1; i += RB)
+      if (tb + i < te) locate(tb + i);
     __syncthreads();
-    uint32_t masks[NST];
 #pragma unroll
     for (int i = 0; i < NST - 1; ++i)
-      masks[i] = kt + DKT * i < ke ? stage(lds0 + i * D_STAGE, kt + DKT * i, p0) : 0;
-    for (int k0 = kt; k0 < ke; k0 += DKT) {
-      const int t = (k0 - kt) / DKT;
+      if (tb + i < te) stage(tb + i);
+    for (int t = tb; t < te; ++t) {
       const uint32_t cur = lds0 + (t % NST) * D_STAGE;
-      // this wave's part of the tile has arrived; behind the barrier every wave's has, and every
-      // wave is done with the tile before, whose stage is filled next
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      // this wave's part of the tile has arrived (the NST - 2 tiles behind it may be in flight);
+      // behind the barrier every wave's has, and every wave is done with the tile before, whose
+      // stage is filled next
+      if (NST > 2 && t + NST - 2 < te) {
+        constexpr int n = (NST - 2) * (DKT / RB);
+        if (w < DKT / 8) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(n + NST - 2) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(n) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      }
       __builtin_amdgcn_s_barrier();
-      const int kn = k0 + DKT * (NST - 1);
-      const uint32_t vm = masks[0];
+      if (t + NST - 1 < te) stage(t + NST - 1);
+      const uint32_t vm = __builtin_amdgcn_readfirstlane(mask_of[t % D_RING]);
+      if (vm != 0) {
+        // S^T: register j of tile u = key 16 u + 4 q + j of the lane's row
+        // (the two tiles in turn, so that a product does not wait for the one before it). K fragments
+        // are read D_AHEAD products ahead; the scheduling barriers keep the compiler to that order
+        // (left alone it waits for each read right before its product)
+        v4f_t s[2] = {zero, zero};
+        const uint32_t kb = cur + ka, rp = cur + ra;
+        auto kfrag = [&](int f) {  // product f: k-step f / 2 of tile f & 1
+          const int kk = f >> 1, u = f & 1;
+          return kk < 16 ? lds_read16((kb ^ (64 * (kk & 3))) + 256 * (kk >> 2) + 16384 * u)
+                         : lds_read16((rp ^ (64 * (kk - 16))) + 2048 * u);
+        };
+        v8s_t kf[D_AHEAD];
 #pragma unroll
-      for (int i = 0; i < NST - 2; ++i) masks[i] = masks[i + 1];
-      masks[NST - 2] = kn < ke ? stage(lds0 + ((t + NST - 1) % NST) * D_STAGE, kn, p0) : 0;
-      if (vm == 0) continue;
+        for (int f = 0; f < D_AHEAD; ++f) kf[f] = kfrag(f);
+#pragma unroll
+        for (int f = 0; f < 36; ++f) {
+          s[f & 1] = mfma16<DT>(kf[f % D_AHEAD], qf[f >> 1], s[f & 1]);
+          if (f + D_AHEAD < 36) kf[f % D_AHEAD] = kfrag(f + D_AHEAD);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        // keys this lane's row sees: bit = key offset in the tile
+        const int d = pos - DKT * t;
+        const uint32_t see = vm & (d >= 31 ? ~0u : d < 0 ? 0u : (2u << d) - 1);
+        if (!__all(see == ~0u)) {
+          const uint32_t sh = see >> (4 * q);
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (!((sh >> (16 * u + j)) & 1)) s[u][j] = -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mx = fmaxf(mx, s[j >> 2][j & 3]);
+        mx = row_max(mx) * a.sl2;
+        if (__any(mx > m + 8.f)) {  // as in k_mla_fwd
+          const float mn = mx > m + 8.f ? mx : m;
+          const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+          l *= alpha;
+          m = mn;
+#pragma unroll
+          for (int dt = 0; dt < 32; ++dt) o[dt] *= alpha;
+        }
+        const float msub = m == -INFINITY ? 0.f : m;
+        float rsum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float p = __builtin_amdgcn_exp2f(__fmaf_rn(s[j >> 2][j & 3], a.sl2, -msub));
+          s[j >> 2][j & 3] = p;
+          rsum += p;
+        }
+        l += row_sum(rsum);
+        v8s_t pf;
+        uint32_t* pw = reinterpret_cast<uint32_t*>(&pf);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          pw[j] = pack_dt<DT>(s[j >> 1][2 * (j & 1)], s[j >> 1][2 * (j & 1) + 1]);
+        const uint32_t vb = cur + va;
+        auto vfrag = [&](int dt) {
+          const uint32_t ad = (vb ^ (32 * (dt & 7))) + 256 * (dt >> 3);
+          const v4s_t lo = lds_read_tr(ad), hi = lds_read_tr(ad + 16384);
+          return (v8s_t){lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        };
+        v8s_t vf[D_AHEAD];
+#pragma unroll
+        for (int dt = 0; dt < D_AHEAD; ++dt) vf[dt] = vfrag(dt);
+#pragma unroll
+        for (int dt = 0; dt < 32; ++dt) {
+          o[dt] = mfma16<DT>(vf[dt % D_AHEAD], pf, o[dt]);
+          if (dt + D_AHEAD < 32) vf[dt % D_AHEAD] = vfrag(dt + D_AHEAD);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      // the addresses of the tile staged in the iteration after next (in the ring's slot of a
+      // tile that every wave has finished), by the waves in turn
+      if (t + NST + 1 < te && w == t % RB) locate(t + NST + 1);
+    }
+    }
 
-      // S^T: register j of tile u = key 16 u + 4 q + j of the lane's row
-      v4f_t s[2] = {zero, zero};
+    if (rb < a.nrb) {
+      if (t0 == 0 && t1 == nt) {  // the whole line of keys: finished
+        const float il = l == 0.f ? 0.f : 1.f / l;  // a row without a key: zeros
+        const int row = D_ROWS * rb + (threadIdx.x & 15);
+        if (row < rows) {
+          uint16_t* op = a.out + ((int64_t)b * rows + row) * DL;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+          for (int dt = 0; dt < 32; ++dt) {
+            uint2 pk;
+            pk.x = pack_dt<DT>(o[dt][0] * il, o[dt][1] * il);
+            pk.y = pack_dt<DT>(o[dt][2] * il, o[dt][3] * il);
+            *reinterpret_cast<uint2*>(op + 16 * dt + 4 * q) = pk;
+          }
+        }
+      } else {
+        const int64_t slot = (2 * (int64_t)wg + (at == begin ? 0 : 1)) * RB + w;
+        if (q == 0) {
+          a.ml[(slot * D_ROWS + c) * 2] = m;
+          a.ml[(slot * D_ROWS + c) * 2 + 1] = l;
+        }
+        v4f_t* pt = reinterpret_cast<v4f_t*>(a.part + slot * D_PART);
 #pragma unroll
-        for (int kk = 0; kk < 16; ++kk)
-          s[u] = mfma16<DT>(
-              lds_read16(((cur + ka) ^ (64 * (kk & 3))) + 256 * (kk >> 2) + 16384 * u), qf[kk],
-              s[u]);
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-          s[u] = mfma16<DT>(lds_read16(((cur + ra) ^ (64 * kk)) + 2048 * u), qf[16 + kk], s[u]);
-      }
-      // keys this lane's row sees: bit = key offset in the tile
-      const int d = pos - k0;
-      const uint32_t see = vm & (d >= 31 ? ~0u : d < 0 ? 0u : (2u << d) - 1);
-      if (!__all(see == ~0u)) {
-        const uint32_t sh = see >> (4 * q);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (!((sh >> (16 * u + j)) & 1)) s[u][j] = -INFINITY;
-      }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) mx = fmaxf(mx, s[j >> 2][j & 3]);
-      mx = row_max(mx) * a.sl2;
-      const float mn = fmaxf(m, mx);
-      const float alpha = (mn == -INFINITY) ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      const float msub = (mn == -INFINITY) ? 0.f : mn;
-      float rsum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float p = __builtin_amdgcn_exp2f(__fmaf_rn(s[j >> 2][j & 3], a.sl2, -msub));
-        s[j >> 2][j & 3] = p;
-        rsum += p;
-      }
-      rsum = row_sum(rsum);
-      l = l * alpha + rsum;
-      m = mn;
-      if (!__all(alpha == 1.f)) {
-#pragma unroll
-        for (int dt = 0; dt < 32; ++dt) o[dt] *= alpha;
-      }
-      v8s_t pf;
-      uint32_t* pw = reinterpret_cast<uint32_t*>(&pf);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        pw[j] = pack_dt<DT>(s[j >> 1][2 * (j & 1)], s[j >> 1][2 * (j & 1) + 1]);
-#pragma unroll
-      for (int dt = 0; dt < 32; ++dt) {
-        const uint32_t at = ((cur + va) ^ (32 * (dt & 7))) + 256 * (dt >> 3);
-        const v4s_t lo = lds_read_tr(at), hi = lds_read_tr(at + 16384);
-        const v8s_t vf = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        o[dt] = mfma16<DT>(vf, pf, o[dt]);
+        for (int dt = 0; dt < 32; ++dt) pt[dt * 64 + lane] = o[dt];
       }
     }
-  }
-  if (rb >= a.nrb) return;
-  if (a.nsplit == 1) {
-    const float il = l == 0.f ? 0.f : 1.f / l;  // a row without a key: zeros
-    if (live) {
-      uint16_t* op = a.out + ((int64_t)b * rows + row) * DL;
-#pragma unroll
-      for (int dt = 0; dt < 32; ++dt) {
-        uint2 pk;
-        pk.x = pack_dt<DT>(o[dt][0] * il, o[dt][1] * il);
-        pk.y = pack_dt<DT>(o[dt][2] * il, o[dt][3] * il);
-        *reinterpret_cast<uint2*>(op + 16 * dt + 4 * q) = pk;
-      }
+    at += t1 - t0;
+    if (y == a.ny - 1 && t1 == nt) {
+      first += nt * a.ny;
+      ++b;
     }
-    return;
   }
-  if (kbeg >= len && sp > 0) return;  // the join reads only the splits a length reaches
-  const int64_t at = ((int64_t)sp * a.B + b) * a.nrb + rb;
-  if (q == 0) {
-    a.ml[(at * D_ROWS + c) * 2] = m;
-    a.ml[(at * D_ROWS + c) * 2 + 1] = l;
-  }
-  v4f_t* pt = reinterpret_cast<v4f_t*>(a.part + at * D_PART);
-#pragma unroll
-  for (int dt = 0; dt < 32; ++dt) pt[dt * 64 + lane] = o[dt];
 }
 
-// Joins the splits of one row block in split order: 8 workgroups of 256 threads per block, a thread
-// one float4 (4 dims of a row) of every split.
-template <int DT>
+// Joins the partial outputs of one row block in key order: 8 workgroups of 256 threads per block, a
+// thread one float4 (4 dims of a row) of every partial.
+template <int DT, int RB>
 __global__ void __launch_bounds__(256) k_mla_join(MlaDecArgs a) {
   const int b = blockIdx.y, rb = blockIdx.x >> 3;
+  const int y = rb / RB, w = rb - y * RB;
+  const int total = dec_total(a), step = dec_step(a, total);
+  int s = 0;
+  {
+    const int lane = threadIdx.x & 63;
+    for (int i = lane; i < b; i += 64) s += dec_tiles(a, i);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
+    s *= a.ny;
+  }
+  const int nt = dec_tiles(a, b);
+  s = __builtin_amdgcn_readfirstlane(s) + y * nt;          // this block's first tile
+  const int i0 = s / step, i1 = (s + nt - 1) / step;       // the workgroups that hold its tiles
+  if (i0 == i1) return;                                    // finished by its workgroup
   const int at4 = (blockIdx.x & 7) * 256 + threadIdx.x;  // float4 of the block: dt * 64 + lane
   const int lane = at4 & 63, c = lane & 15, q = lane >> 4, dt = at4 >> 6;
   const int row = D_ROWS * rb + c, rows = a.Sq * a.H;
   if (row >= rows) return;
-  const int len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.nb * a.ps);
-  const int ns = max(1, (len + a.chunk - 1) / a.chunk);
-  const int64_t step = (int64_t)a.B * a.nrb, at = (int64_t)b * a.nrb + rb;
-  float m = -INFINITY;
-  for (int s = 0; s < ns; ++s) m = fmaxf(m, a.ml[((s * step + at) * D_ROWS + c) * 2]);
-  float l = 0.f;
+  // slot of workgroup i's segment: its second only where its range began before this block
+  auto slot = [&](int i) { return (2 * (int64_t)i + (i == i0 && i0 * step < s ? 1 : 0)) * RB + w; };
+  float m = -INFINITY, l = 0.f;
   v4f_t acc = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < ns; ++s) {
-    const int64_t i = s * step + at;
-    const float ms = a.ml[(i * D_ROWS + c) * 2];
-    // a NaN partial (fmaxf passes it by) must reach the result
-    const float f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - m);
-    l += f * a.ml[(i * D_ROWS + c) * 2 + 1];
-    acc += f * reinterpret_cast<const v4f_t*>(a.part + i * D_PART)[at4];
+  // four partials in flight; the running maximum rescales (a NaN partial reaches the result)
+  for (int i = i0; i <= i1; i += 4) {
+    float ms[4], ls[4];
+    v4f_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t at = slot(min(i + j, i1));
+      ms[j] = a.ml[(at * D_ROWS + c) * 2];
+      ls[j] = a.ml[(at * D_ROWS + c) * 2 + 1];
+      v[j] = reinterpret_cast<const v4f_t*>(a.part + at * D_PART)[at4];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i + j > i1 || ms[j] == -INFINITY) continue;
+      const float mn = fmaxf(m, ms[j]);
+      const float f0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      const float f1 = __builtin_amdgcn_exp2f(ms[j] - mn);
+      l = l * f0 + ls[j] * f1;
+      acc = acc * f0 + v[j] * f1;
+      m = mn;
+    }
   }
   const float il = l == 0.f ? 0.f : 1.f / l;
   uint2 pk;
@@ -515,40 +695,33 @@ __global__ void __launch_bounds__(256) k_mla_join(MlaDecArgs a) {
 }
 
 struct DecPlan {
-  int rb, nrb, nsplit, chunk;
+  int rb, nrb, ny, wgs;
 };
-// RB row blocks per workgroup (all heads of a token share its key tiles); the keys split until
-// about two workgroups per CU exist, no split below 128 keys
+// RB row blocks per workgroup (all heads of a token share its key tiles); as many workgroups as the
+// chip holds at once: one of 8 waves per CU (144 KB of stages), two of fewer
 DecPlan dec_plan(int64_t B, int64_t rows, int64_t maxlen) {
   DecPlan p;
   p.nrb = (int)((rows + D_ROWS - 1) / D_ROWS);
   p.rb = p.nrb <= 1 ? 1 : p.nrb <= 2 ? 2 : p.nrb <= 4 ? 4 : 8;
-  const int64_t wgs = B * ((p.nrb + p.rb - 1) / p.rb);
-  int64_t ns = (512 + wgs - 1) / wgs;
-  const int64_t most = (maxlen + 127) / 128;
-  if (ns > most) ns = most;
-  if (ns < 1) ns = 1;
-  p.chunk = (int)(((maxlen + ns - 1) / ns + DKT - 1) / DKT * DKT);
-  if (p.chunk < DKT) p.chunk = DKT;
-  p.nsplit = (int)((maxlen + p.chunk - 1) / p.chunk);
-  if (p.nsplit < 1) p.nsplit = 1;
+  p.ny = (p.nrb + p.rb - 1) / p.rb;
+  const int64_t most = (B * p.ny * ((maxlen + DKT - 1) / DKT) + D_MIN - 1) / D_MIN;
+  const int64_t fit = p.rb == 8 ? 256 : 512;
+  p.wgs = (int)(most < fit ? most : fit);
   return p;
 }
 
 template <int DT, int RB, int NST>
 int launch_dec(const MlaDecArgs& a, hipStream_t st) {
-  constexpr int lds = NST * D_STAGE + (D_TAB + 1) * 4;
+  constexpr int lds = NST * D_STAGE + D_RING * (DKT * 16 + 4) + (dec_tab(NST) * DKT + 1) * 4;
+  static_assert(lds <= (NST == 4 ? 163840 : 81920), "one / two workgroups per CU");
+  static_assert(NST + 2 <= D_RING, "tiles whose addresses are live");
   (void)hipFuncSetAttribute((const void*)k_mla_dec<DT, RB, NST>,
                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  hipLaunchKernelGGL((k_mla_dec<DT, RB, NST>),
-                     dim3((unsigned)a.nsplit, (unsigned)((a.nrb + RB - 1) / RB), (unsigned)a.B),
-                     64 * RB, lds, st, a);
+  hipLaunchKernelGGL((k_mla_dec<DT, RB, NST>), dim3((unsigned)a.wgs), 64 * RB, lds, st, a);
   if (int rc = check_launch("lcq_mla_decode")) return rc;
-  if (a.nsplit > 1) {
-    hipLaunchKernelGGL(k_mla_join<DT>, dim3((unsigned)a.nrb * 8, (unsigned)a.B), 256, 0, st, a);
-    return check_launch("lcq_mla_decode");
-  }
-  return LCQ_OK;
+  if (a.wgs == 1) return LCQ_OK;
+  hipLaunchKernelGGL((k_mla_join<DT, RB>), dim3((unsigned)a.nrb * 8, (unsigned)a.B), 256, 0, st, a);
+  return check_launch("lcq_mla_decode");
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -621,7 +794,7 @@ extern "C" int64_t lcq_mla_decode_workspace_bytes(int64_t B, int64_t Sq, int64_t
                                                   int64_t max_len) {
   if (B <= 0 || Sq <= 0 || H <= 0 || max_len <= 0) return 0;
   const DecPlan p = dec_plan(B, Sq * H, max_len);
-  return p.nsplit == 1 ? 0 : (int64_t)p.nsplit * B * p.nrb * (D_PART + 2 * D_ROWS) * 4;
+  return p.wgs == 1 ? 0 : 2 * (int64_t)p.wgs * p.rb * (D_PART + 2 * D_ROWS) * 4;
 }
 
 extern "C" int lcq_mla_decode(const void* q_latent, const int64_t* q_latent_strides,
@@ -648,6 +821,7 @@ extern "C" int lcq_mla_decode(const void* q_latent, const int64_t* q_latent_stri
   LCQ_REQUIRE(al16(q_latent) && al16(q_rope) && al16(ckv) && al16(k_rope) && al16(out),
               "16-byte aligned tensors required");
   const DecPlan p = dec_plan(B, Sq * H, nb * page_size);
+  LCQ_REQUIRE(B * p.ny * ((nb * page_size + DKT - 1) / DKT) < (int64_t(1) << 30), "cache too long");
   const int64_t need = lcq_mla_decode_workspace_bytes(B, Sq, H, nb * page_size);
   LCQ_REQUIRE(ws_bytes >= need && (need == 0 || (workspace && al16(workspace))),
               "workspace too small (lcq_mla_decode_workspace_bytes)");
@@ -665,9 +839,9 @@ extern "C" int lcq_mla_decode(const void* q_latent, const int64_t* q_latent_stri
   a.out = static_cast<uint16_t*>(out);
   a.P = pages;
   a.B = (int)B; a.Sq = (int)Sq; a.H = (int)H; a.ps = (int)page_size; a.nb = (int)nb;
-  a.nrb = p.nrb; a.chunk = p.chunk; a.nsplit = p.nsplit;
+  a.nrb = p.nrb; a.ny = p.ny; a.wgs = p.wgs;
   a.part = static_cast<float*>(workspace);
-  a.ml = a.part ? a.part + (int64_t)p.nsplit * B * p.nrb * D_PART : nullptr;
+  a.ml = a.part ? a.part + 2 * (int64_t)p.wgs * p.rb * D_PART : nullptr;
   a.sl2 = scale * 1.44269504088896340736f;
   hipStream_t st = as_stream(stream);
   auto go = [&](auto dt) {
