@@ -761,14 +761,17 @@ int lcq_int4_gemm_grouped(const void* x, int dtype, int64_t ldx, int64_t x_rows,
  * NULL: Skv - Sq), kv_lens int32 [B] (device; NULL: Skv; clamped to [0, Skv]). Keys at or past
  * kv_lens are not read; those below must be finite (a NaN or an infinity there can reach rows that
  * do not see the key). out [B, Sq, H, 128] contiguous. Key / value seq strides in [0, 2^24).
+ * workspace: lcq_mla_fwd_causal_workspace_bytes(B, H, Sq, Skv) bytes (0 unless few query tiles have
+ * their keys split; the shares are joined in a fixed order: the same call gives the same bits).
  * ------------------------------------------------------------------------------------- */
+int64_t lcq_mla_fwd_causal_workspace_bytes(int64_t B, int64_t H, int64_t Sq, int64_t Skv);
 int lcq_mla_fwd_causal(const void* q_nope, const int64_t* q_nope_strides, const void* q_rope,
                        const int64_t* q_rope_strides, const void* k_nope,
                        const int64_t* k_nope_strides, const void* k_rope,
                        const int64_t* k_rope_strides, const void* v, const int64_t* v_strides,
                        int dtype, int64_t B, int64_t H, int64_t Sq, int64_t Skv,
                        const int32_t* q_start, const int32_t* kv_lens, float scale, void* out,
-                       void* stream);
+                       void* workspace, int64_t ws_bytes, void* stream);
 
 /* Absorbed, over a paged latent cache (decode): out[b, i, h] = sum_j softmax_j((q_latent_i . c_j +
  * q_rope_i . r_j) scale) c_j (512 dims) over the cached tokens j <= kv_lens[b] - Sq + i. Token j

@@ -150,7 +150,8 @@ SIGNATURES = {
     'lcq_int4_gemm_grouped': ([_vp, _int, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _int, _int,
                                _int, _i64, _i64, _i64, _vp, _vp], _int),
     'lcq_mla_fwd_causal': ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64,
-                            _i64, _i64, _vp, _vp, _f32, _vp, _vp], _int),
+                            _i64, _i64, _vp, _vp, _f32, _vp, _vp, _i64, _vp], _int),
+    'lcq_mla_fwd_causal_workspace_bytes': ([_i64, _i64, _i64, _i64], _i64),
     'lcq_mla_decode_workspace_bytes': ([_i64, _i64, _i64, _i64], _i64),
     'lcq_mla_decode': ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _int,
                         _i64, _i64, _i64, _f32, _vp, _vp, _i64, _vp], _int),

@@ -50,6 +50,8 @@ constexpr int FQT = 128;  // query rows per workgroup (4 waves of 32)
 constexpr int FKT = 64;   // keys per tile
 constexpr int F_STAGE = FKT * (DN + DR + DV) * 2;  // 40 KB
 constexpr int F_AHEAD = 6;                         // LDS fragments read ahead of their product
+constexpr int F_MIN = 8;                           // least tiles of a share of the keys
+constexpr int F_PART = FQT * DV;                   // floats of a query tile's partial output
 
 struct MlaFwdArgs {
   const uint16_t *qn, *qr, *kn, *kr, *v;
@@ -57,7 +59,9 @@ struct MlaFwdArgs {
   int64_t qnb, qnh, qns, qrb, qrh, qrs, knb, knh, kns, krb, krs, vb, vh, vs;  // elements
   const int32_t* q_start;   // nullable [B]: position of query 0 (default Skv - Sq)
   const int32_t* kv_lens;   // nullable [B]: valid keys (default Skv)
-  int Sq, Skv, H, nqt;
+  int Sq, Skv, H, nqt, ns;  // ns shares of the keys per query tile
+  float* part;              // ns > 1: [query tiles][ns] partial outputs, then their max / sum
+  float2* ml;
   float sl2;                // scale * log2(e)
 };
 
@@ -93,7 +97,9 @@ struct FwdStage {
   }
 };
 
-template <int DT>
+// SPLIT: the workgroup takes its share of the query tile's key tiles and leaves the unnormalised
+// output (lane order) with the rows' max and sum for k_mla_fwd_join
+template <int DT, bool SPLIT>
 __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char mla_lds[];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -107,11 +113,24 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
     L = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (p >> 3);
   }
   const int qt = a.nqt - 1 - L % a.nqt;  // longest tiles first
-  const int hq = (L / a.nqt) % a.H, b = L / (a.nqt * a.H);
+  const int sp = SPLIT ? (L / a.nqt) % a.ns : 0;
+  if (SPLIT) L /= a.ns * a.nqt;
+  else L /= a.nqt;
+  const int hq = L % a.H, b = L / a.H;
   const int q0 = qt * FQT;
   const int klen = a.kv_lens ? min(max(a.kv_lens[b], 0), a.Skv) : a.Skv;
   const int qs = a.q_start ? min(max(a.q_start[b], -(1 << 29)), 1 << 29) : a.Skv - a.Sq;
-  const int kend = min(klen, qs + q0 + FQT);
+  int kbeg = 0, kend = min(klen, qs + min(q0 + FQT, a.Sq));
+  const int64_t pt = SPLIT ? ((int64_t)(b * a.H + hq) * a.nqt + qt) * a.ns + sp : 0;
+  if constexpr (SPLIT) {
+    const int n = kend > 0 ? (kend + FKT - 1) / FKT : 0, each = (n + a.ns - 1) / a.ns;
+    kbeg = min(sp * each * FKT, max(kend, 0));
+    kend = min(kbeg + each * FKT, kend);
+    if (kbeg >= kend) {  // nothing to add: the join skips rows of sum 0
+      if (tid < FQT) a.ml[pt * FQT + tid] = make_float2(-INFINITY, 0.f);
+      return;
+    }
+  }
   if (kend <= 0) {  // no row of the tile sees a key
     for (int i = tid; i < FQT * 16; i += 256) {
       const int qr = q0 + (i >> 4);
@@ -127,13 +146,13 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
   const uint16_t* krp = uni(a.kr + b * a.krb);
   const uint16_t* vp = uni(a.v + b * a.vb + hq * a.vh);
   FwdStage fs;
-  fs.init(a, min(FKT - 1, klen - 1), w, lane);
+  fs.init(a, min(FKT - 1, klen - 1 - kbeg), w, lane);
   auto stage = [&](int k0, int buf) {  // called for tile after tile
-    if (k0 > 0 && klen - 1 - k0 < FKT - 1) fs.init(a, klen - 1 - k0, w, lane);
+    if (k0 > kbeg && klen - 1 - k0 < FKT - 1) fs.init(a, klen - 1 - k0, w, lane);
     fs.issue(lds0 + buf * F_STAGE, uni(knp + k0 * a.kns), uni(krp + k0 * a.krs),
              uni(vp + k0 * a.vs), w);
   };
-  stage(0, 0);
+  stage(kbeg, 0);
 
   const int qrow = q0 + 32 * w + c;  // this lane's query row (both halves)
   // Q^T as the B operand of mfma(K, Q^T): lane holds Q[qrow][16 kk + 8 h + j]
@@ -147,7 +166,9 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
                  : qrp + qrow * a.qrs + 16 * (kk - 8) + 8 * h);
   }
   const int pos = min(qs + qrow, klen - 1);       // last key this lane's row sees
-  const int wmin = min(qs + q0 + 32 * w, klen - 1);  // the least of the wave's rows
+  // the least and the greatest of the wave's rows (a wave without rows: none)
+  const int wmin = min(qs + q0 + 32 * w, klen - 1);
+  const int wmax = q0 + 32 * w < a.Sq ? min(qs + q0 + 32 * w + 31, klen - 1) : -1;
   float m = -INFINITY, l = 0.f;
   v16f_t o[4];
 #pragma unroll
@@ -162,13 +183,14 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
                       16 * ((2 * (g & 1) + (pp >> 1)) ^ (qq << 2 | (g >> 1))) + 8 * (pp & 1);
 
   int it = 0;
-  for (int k0 = 0; k0 < kend; k0 += FKT, ++it) {
+  for (int k0 = kbeg; k0 < kend; k0 += FKT, ++it) {
     const uint32_t cur = lds0 + (it & 1) * F_STAGE;
     // this wave's part of the tile has arrived; behind the barrier every wave's has, and every
     // wave is done with the tile before, whose stage is filled next
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     if (k0 + FKT < kend) stage(k0 + FKT, (it & 1) ^ 1);
+    if (k0 > wmax) continue;  // no row of this wave sees the tile
 
     // S^T tiles t: register r holds key k0 + 32 t + (r & 3) + 8 (r >> 2) + 4 h of the lane's row.
     // The two tiles in turn, so that a product does not wait for the one before it; K fragments
@@ -259,6 +281,17 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
       }
     }
   }
+  if constexpr (SPLIT) {
+    float4* dst = reinterpret_cast<float4*>(a.part + pt * F_PART) + tid;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        dst[(4 * dt + i) * 256] = make_float4(o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2],
+                                              o[dt][4 * i + 3]);
+    if (h == 0) a.ml[pt * FQT + 32 * w + c] = make_float2(m, l);
+    return;
+  }
   __syncthreads();
   // a row that saw no key has l = 0: zeros (a NaN l stays one)
   const float il = l == 0.f ? 0.f : 1.f / l;
@@ -283,6 +316,83 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
       *reinterpret_cast<uint4*>(a.out + (((int64_t)b * a.Sq + qr) * a.H + hq) * DV + ch * 8) =
           *reinterpret_cast<const uint4*>(mla_lds + img_off(row, ch));
   }
+}
+
+// Joins the shares of a query tile, 32 dims (one dt of k_mla_fwd) per workgroup, in share order.
+template <int DT>
+__global__ void __launch_bounds__(256) k_mla_fwd_join(MlaFwdArgs a) {
+  __shared__ __attribute__((aligned(16))) char img[FQT * 64];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 31, h = lane >> 5;
+  const int dt = blockIdx.x & 3, tile = blockIdx.x >> 2;
+  const int qt = tile % a.nqt, hq = (tile / a.nqt) % a.H, b = tile / (a.nqt * a.H);
+  const float2* ml = a.ml + (int64_t)tile * a.ns * FQT + 32 * w + c;
+  float M = -INFINITY;
+  for (int i = 0; i < a.ns; ++i) M = fmaxf(M, ml[i * FQT].x);
+  const float msub = M == -INFINITY ? 0.f : M;
+  float l = 0.f, acc[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+  const float4* pt =
+      reinterpret_cast<const float4*>(a.part + (int64_t)tile * a.ns * F_PART) + 4 * dt * 256 + tid;
+  for (int i = 0; i < a.ns; ++i, pt += F_PART / 4) {
+    const float2 p = ml[i * FQT];
+    if (p.y == 0.f) continue;  // the row saw no key there, and the share may not be written
+    const float f = __builtin_amdgcn_exp2f(p.x - msub);
+    l += f * p.y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 v = pt[j * 256];
+      acc[4 * j] += f * v.x;
+      acc[4 * j + 1] += f * v.y;
+      acc[4 * j + 2] += f * v.z;
+      acc[4 * j + 3] += f * v.w;
+    }
+  }
+  const float il = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {  // dims 8 j + 4 h ..
+    uint2 pk;
+    pk.x = pack_dt<DT>(acc[4 * j] * il, acc[4 * j + 1] * il);
+    pk.y = pack_dt<DT>(acc[4 * j + 2] * il, acc[4 * j + 3] * il);
+    *reinterpret_cast<uint2*>(img + 64 * (32 * w + c) + 16 * j + 8 * h) = pk;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int idx = i * 256 + tid, row = idx >> 2, ch = idx & 3, qr = qt * FQT + row;
+    if (qr < a.Sq)
+      *reinterpret_cast<uint4*>(a.out + (((int64_t)b * a.Sq + qr) * a.H + hq) * DV + 32 * dt +
+                                8 * ch) = *reinterpret_cast<const uint4*>(img + 64 * row + 16 * ch);
+  }
+}
+
+// Shares of the keys per query tile. Two workgroups fit a CU; when the query tiles fill at most
+// half of those 512 places, their keys are split, F_MIN tiles at least to a share: a chunk of 77
+// rows of 128 heads over 4 Ki keys takes 79 us, 145 without shares (96 with one per CU).
+int fwd_shares(int64_t B, int64_t H, int64_t Sq, int64_t Skv) {
+  const int64_t tiles = B * H * ((Sq + FQT - 1) / FQT);
+  const int64_t most = (Skv + FKT - 1) / FKT / F_MIN, fit = 512 / tiles;
+  const int64_t n = most < fit ? most : fit;
+  return n < 1 ? 1 : (int)n;
+}
+
+template <int DT>
+int launch_fwd(const MlaFwdArgs& a, int64_t tiles, hipStream_t st) {
+  constexpr int lds = 2 * F_STAGE;
+  auto go = [&](auto split) {
+    constexpr bool SP = decltype(split)::value;
+    (void)hipFuncSetAttribute((const void*)k_mla_fwd<DT, SP>,
+                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    hipLaunchKernelGGL((k_mla_fwd<DT, SP>), dim3((unsigned)(tiles * a.ns)), 256, lds, st, a);
+  };
+  if (a.ns == 1) {
+    go(std::false_type{});
+    return check_launch("lcq_mla_fwd_causal");
+  }
+  go(std::true_type{});
+  if (int rc = check_launch("lcq_mla_fwd_causal")) return rc;
+  hipLaunchKernelGGL(k_mla_fwd_join<DT>, dim3((unsigned)(tiles * 4)), 256, 0, st, a);
+  return check_launch("lcq_mla_fwd_causal");
 }
 
 // ---------------------------------------------------------------------------------------
@@ -731,13 +841,23 @@ bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 using namespace lcq;
 
+extern "C" int64_t lcq_mla_fwd_causal_workspace_bytes(int64_t B, int64_t H, int64_t Sq,
+                                                      int64_t Skv) {
+  if (B <= 0 || H <= 0 || Sq <= 0 || Skv <= 0 || B >= (1 << 24) || H >= (1 << 24) ||
+      B * H >= (int64_t(1) << 31) || Sq >= (1 << 28) || Skv >= (1 << 28))
+    return 0;
+  const int64_t ns = fwd_shares(B, H, Sq, Skv);
+  return ns == 1 ? 0 : B * H * ((Sq + FQT - 1) / FQT) * ns * (F_PART + 2 * FQT) * 4;
+}
+
 extern "C" int lcq_mla_fwd_causal(const void* q_nope, const int64_t* q_nope_strides,
                                   const void* q_rope, const int64_t* q_rope_strides,
                                   const void* k_nope, const int64_t* k_nope_strides,
                                   const void* k_rope, const int64_t* k_rope_strides,
                                   const void* v, const int64_t* v_strides, int dtype, int64_t B,
                                   int64_t H, int64_t Sq, int64_t Skv, const int32_t* q_start,
-                                  const int32_t* kv_lens, float scale, void* out, void* stream) {
+                                  const int32_t* kv_lens, float scale, void* out, void* workspace,
+                                  int64_t ws_bytes, void* stream) {
   LCQ_REQUIRE(dtype == LCQ_BF16 || dtype == LCQ_F16, "bf16 / fp16 only");
   LCQ_REQUIRE(B >= 0 && H > 0 && Sq >= 0 && Skv > 0, "bad shape");
   LCQ_REQUIRE(Sq < (1 << 28) && Skv < (1 << 28), "sequence too long");
@@ -748,7 +868,8 @@ extern "C" int lcq_mla_fwd_causal(const void* q_nope, const int64_t* q_nope_stri
               "null pointer");
   LCQ_REQUIRE(q_start || Skv >= Sq, "more queries than keys needs q_start");
   const int64_t nqt = (Sq + FQT - 1) / FQT;
-  LCQ_REQUIRE(B < (1 << 24) && H < (1 << 24) && B * H * nqt < (int64_t(1) << 31),
+  LCQ_REQUIRE(B < (1 << 24) && H < (1 << 24) && B * H < (int64_t(1) << 31) &&
+                  B * H * nqt < (int64_t(1) << 31),
               "shape too large");
   int64_t all = 0;
   for (int i = 0; i < 3; ++i)
@@ -776,18 +897,16 @@ extern "C" int lcq_mla_fwd_causal(const void* q_nope, const int64_t* q_nope_stri
   a.kv_lens = kv_lens;
   a.Sq = (int)Sq; a.Skv = (int)Skv; a.H = (int)H; a.nqt = (int)nqt;
   a.sl2 = scale * 1.44269504088896340736f;
-  constexpr int lds = 2 * F_STAGE;
-  const dim3 grid((unsigned)(B * H * nqt));
-  if (dtype == LCQ_BF16) {
-    (void)hipFuncSetAttribute((const void*)k_mla_fwd<LCQ_BF16>,
-                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    hipLaunchKernelGGL(k_mla_fwd<LCQ_BF16>, grid, 256, lds, as_stream(stream), a);
-  } else {
-    (void)hipFuncSetAttribute((const void*)k_mla_fwd<LCQ_F16>,
-                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    hipLaunchKernelGGL(k_mla_fwd<LCQ_F16>, grid, 256, lds, as_stream(stream), a);
+  a.ns = fwd_shares(B, H, Sq, Skv);
+  const int64_t need = lcq_mla_fwd_causal_workspace_bytes(B, H, Sq, Skv);
+  LCQ_REQUIRE(ws_bytes >= need && (need == 0 || (workspace && al16(workspace))),
+              "workspace too small (lcq_mla_fwd_causal_workspace_bytes)");
+  if (a.ns > 1) {
+    a.part = static_cast<float*>(workspace);
+    a.ml = reinterpret_cast<float2*>(a.part + B * H * nqt * a.ns * F_PART);
   }
-  return check_launch("lcq_mla_fwd_causal");
+  return dtype == LCQ_BF16 ? launch_fwd<LCQ_BF16>(a, B * H * nqt, as_stream(stream))
+                           : launch_fwd<LCQ_F16>(a, B * H * nqt, as_stream(stream));
 }
 
 extern "C" int64_t lcq_mla_decode_workspace_bytes(int64_t B, int64_t Sq, int64_t H,

@@ -1621,13 +1621,15 @@ def mla_fwd_causal(q_nope: torch.Tensor, q_rope: torch.Tensor, k_nope: torch.Ten
     kr = _mla_rows('k_rope', k_rope, (B, Skv, MLA_ROPE))
     vv = _mla_rows('v', v, (B, H, Skv, MLA_V))
     out = qn.new_empty((B, Sq, H, MLA_V))
+    wsb = N.load().lcq_mla_fwd_causal_workspace_bytes(B, H, Sq, Skv)
+    ws = qn.new_empty(wsb, dtype=torch.uint8) if wsb else None
     keep, st = _strides(qn, qr, kn, kr, vv)
     with N.on_device(qn):
         N.call('lcq_mla_fwd_causal', qn.data_ptr(), st[0], qr.data_ptr(), st[1], kn.data_ptr(),
                st[2], kr.data_ptr(), st[3], vv.data_ptr(), st[4], N.dt(qn), B, H, Sq, Skv,
                None if q_start is None else q_start.data_ptr(),
                None if kv_lens is None else kv_lens.data_ptr(), float(scale), out.data_ptr(),
-               N.stream_of(qn))
+               None if ws is None else ws.data_ptr(), wsb, N.stream_of(qn))
     N.note_work('lcq_mla_fwd_causal',
                 2.0 * B * H * Sq * (Skv - (Sq - 1) / 2) * (MLA_NOPE + MLA_ROPE + MLA_V))
     return out

@@ -60,6 +60,33 @@ def test_prefill_padded_and_empty_rows(dev, dt):
     assert (got[:3] == 0).all()
 
 
+@pytest.mark.parametrize('dt', DTYPES)
+@pytest.mark.parametrize('B,H,Sq,Skv', [
+    (1, 1, 1, 1024), (1, 2, 77, 1500), (2, 3, 130, 2049), (1, 16, 200, 1100), (3, 1, 5, 4000)])
+def test_prefill_keys_split(dev, dt, B, H, Sq, Skv):
+    """Few query tiles against many keys: the keys are shared out and joined. Lengths and positions
+    that leave shares, rows and sequences empty; the same call gives the same bits."""
+    from lightcompress_amd import _native as N, ops
+    assert N.load().lcq_mla_fwd_causal_workspace_bytes(B, H, Sq, Skv) > 0
+    g = torch.Generator().manual_seed(B * 100 + H * 10 + Sq + Skv)
+    x = prefill_inputs(g, B, H, Sq, Skv, dt, dev)
+    got = ops.mla_fwd_causal(*x, SCALE)
+    y, tol = R.fwd_causal(*x, SCALE)
+    assert R.close(got, y, tol)
+    assert torch.equal(got, ops.mla_fwd_causal(*x, SCALE))
+    for lens, start in (([Skv] * 3, [3, Skv, -2]), ([65, Skv - 1, 0], [70, 600, 9]),
+                        ([0, 0, 1], [0, 0, 0])):
+        lens, start = (torch.tensor(t[:B], dtype=torch.int32) for t in (lens, start))
+        z = [t.clone() for t in x]
+        for b in range(B):
+            z[2][b, :, int(lens[b]):] = float('nan')
+            z[3][b, int(lens[b]):] = float('inf')
+            z[4][b, :, int(lens[b]):] = float('nan')
+        got = ops.mla_fwd_causal(*z, SCALE, q_start=start.to(dev), kv_lens=lens.to(dev))
+        y, tol = R.fwd_causal(*z, SCALE, q_start=start, kv_lens=lens)
+        assert R.close(got, y, tol)
+
+
 def test_prefill_scores_of_any_size(dev):
     """Scores far from zero (a row's softmax is nearly one key), equal scores, huge scale."""
     from lightcompress_amd import ops
