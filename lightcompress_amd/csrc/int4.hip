@@ -11,6 +11,8 @@
 //
 // Both layouts are read as they were deployed: no second copy of the weights is made or kept.
 #define LCQ_BF16_HW 1
+#include <type_traits>
+
 #include "int4_common.h"
 
 namespace lcq {
@@ -109,7 +111,8 @@ __device__ __forceinline__ void i4_store(const I4Args& a, int64_t row, int64_t c
 
 // column tiles of 16 per workgroup of the 16-row kernel: as many as leave about 200 workgroups (a
 // tile more shares x's fragments and their order changes; measured at 8 x 14336 x 4096: 4 tiles
-// 10.9 us, 2 13.5, 1 19.1; at 1 x 4096 x 4096: 1 tile 5.2 us, 2 6.1, 4 8.1)
+// 10.9 us, 2 13.5, 1 19.1; at 1 x 4096 x 4096: 1 tile 5.2 us, 2 6.1, 4 8.1). Of groups n is all
+// their columns (16 experts of 2048: 4 tiles 22 us, 1 38)
 inline int i4_few_tiles(int layout, int64_t n) {
   return layout == LA || n >= 12288 ? 4 : n >= 6144 ? 2 : 1;
 }
@@ -241,7 +244,10 @@ struct I4Few {
   static constexpr int T = NT * SETS;
   static constexpr bool HALVE = W * MT * T > 64;  // partial tiles of all waves past 64 KB
   static constexpr int WR = HALVE ? W / 2 : W;
-  static constexpr bool PRE = LAYOUT == LA && MT == 1;  // the next unit is loaded meanwhile
+  // the next unit is loaded meanwhile, where its registers cost no occupancy that hides more (one
+  // matrix of vLLM words, MT 1: 5.5 us without, 5.8 with; 64 experts' gate and up: 223 with, 228
+  // without; AutoAWQ, MT 4, 8 waves: 25.5 without, 37.9 with)
+  static constexpr bool PRE = MT == 1 ? LAYOUT == LA || SETS == 2 : LAYOUT == LV && W == 4;
   static constexpr int STAGE = LAYOUT == LA ? 4096 * SETS : 0;
   static constexpr int RED = WR * MT * T * 1024, STAGES = W * (PRE ? 2 : 1) * STAGE;
   static constexpr int LDS = RED > STAGES ? RED : STAGES;
@@ -295,7 +301,7 @@ __global__ __launch_bounds__(64 * W) void k_int4_few(I4Args a) {
   const int sp = a.row_off ? 0 : blockIdx.z;
   const int u0 = nb * sp / a.nsplit, un = nb * (sp + 1) / a.nsplit - u0;
   const int b0 = u0 + un * w / W, b1 = u0 + un * (w + 1) / W;
-  i4_v4u xf[NB][MT][4], wv[SETS][LAYOUT == LV ? NT : 1];
+  i4_v4u xf[NB][MT][4], wv[NB][SETS][LAYOUT == LV ? NT : 1];
   I4Scales<LAYOUT, F> scl[NB][SETS];
   auto load = [&](int slot, int b) {
     const int k0 = b * 128;
@@ -312,7 +318,7 @@ __global__ __launch_bounds__(64 * W) void k_int4_few(I4Args a) {
       for (int s = 0; s < SETS; ++s)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-          wv[s][t] = gload<i4_v4u>(qw[s], cols.wo[t] + kw);
+          wv[slot][s][t] = gload<i4_v4u>(qw[s], cols.wo[t] + kw);
     }
 #pragma unroll
     for (int s = 0; s < SETS; ++s) scl[slot][s].load(a, cols, sc[s], qz[s], k0);
@@ -339,7 +345,7 @@ __global__ __launch_bounds__(64 * W) void k_int4_few(I4Args a) {
 #pragma unroll
         for (int s = 0; s < SETS; ++s)
 #pragma unroll
-          for (int t = 0; t < NT; ++t) wv[s][t] = i4_transpose(wv[s][t]);
+          for (int t = 0; t < NT; ++t) wv[slot][s][t] = i4_transpose(wv[slot][s][t]);
       }
 #pragma unroll
       for (int i = 0; i < MT; ++i)
@@ -349,51 +355,50 @@ __global__ __launch_bounds__(64 * W) void k_int4_few(I4Args a) {
 #pragma unroll
     for (int f = 0; f < F; ++f) {
       if (F > 1 && k0 + 128 / F * f >= a.k) break;
-      i4_v4f g[MT][T], xs[MT];
+      i4_v4f xs[MT];
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         xs[i] = zero;
 #pragma unroll
-        for (int t = 0; t < T; ++t) g[i][t] = zero;
+        for (int j = 4 / F * f; j < 4 / F * (f + 1); ++j)
+          xs[i] = i4_mfma<DT>(xf[slot][i][j], ones, xs[i]);
       }
 #pragma unroll
-      for (int j = 4 / F * f; j < 4 / F * (f + 1); ++j) {
+      for (int s = 0; s < SETS; ++s) {
+        i4_v4u pk[LAYOUT == LA ? 4 / F : 1];
+        if constexpr (LAYOUT == LA) {
+          typedef uint32_t v2u_t __attribute__((ext_vector_type(2)));
 #pragma unroll
-        for (int i = 0; i < MT; ++i) xs[i] = i4_mfma<DT>(xf[slot][i][j], ones, xs[i]);
-#pragma unroll
-        for (int s = 0; s < SETS; ++s) {
-          i4_v4u pk = {0, 0, 0, 0};
-          if constexpr (LAYOUT == LA) {
-            const uint32_t at = tr + slot * C::STAGE + s * 4096 + 1024 * j;
-            const v4s_t lo = lds_read_tr(at), hi = lds_read_tr(at + 128);
-            typedef uint32_t v2u_t __attribute__((ext_vector_type(2)));
-            const v2u_t l = __builtin_bit_cast(v2u_t, lo), h = __builtin_bit_cast(v2u_t, hi);
-            pk = i4_v4u{l.x, l.y, h.x, h.y};
-          }
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const i4_v4u bf = LAYOUT == LV ? i4_word<DT>(wv[s][LAYOUT == LV ? t : 0][j], kc)
-                                           : i4_nibble<DT>(pk, t, kc);
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-              g[i][s * NT + t] = i4_mfma<DT>(xf[slot][i][j], bf, g[i][s * NT + t]);
+          for (int j = 0; j < 4 / F; ++j) {
+            const uint32_t at = tr + slot * C::STAGE + s * 4096 + 1024 * (4 / F * f + j);
+            const v2u_t l = __builtin_bit_cast(v2u_t, lds_read_tr(at));
+            const v2u_t h = __builtin_bit_cast(v2u_t, lds_read_tr(at + 128));
+            pk[j] = i4_v4u{l.x, l.y, h.x, h.y};
           }
         }
-      }
-#pragma unroll
-      for (int s = 0; s < SETS; ++s)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
+          i4_v4f g[MT];
+#pragma unroll
+          for (int i = 0; i < MT; ++i) g[i] = zero;
+#pragma unroll
+          for (int j = 0; j < 4 / F; ++j) {
+            const i4_v4u bf = LAYOUT == LV
+                                  ? i4_word<DT>(wv[slot][s][LAYOUT == LV ? t : 0][4 / F * f + j], kc)
+                                  : i4_nibble<DT>(pk[LAYOUT == LA ? j : 0], t, kc);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) g[i] = i4_mfma<DT>(xf[slot][i][4 / F * f + j], bf, g[i]);
+          }
           float sv, zv;
           scl[slot][s].get(f, t, c, sv, zv);
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              acc[i][s * NT + t][r] =
-                  __fmaf_rn(sv, __fmaf_rn(-zv, xs[i][r], g[i][s * NT + t][r]),
-                            acc[i][s * NT + t][r]);
+              acc[i][s * NT + t][r] = __fmaf_rn(sv, __fmaf_rn(-zv, xs[i][r], g[i][r]),
+                                                acc[i][s * NT + t][r]);
         }
+      }
     }
   };
   if constexpr (C::PRE) {
@@ -796,11 +801,17 @@ bool i4_use_tile(const I4Args& a, int layout, int sets) {
   return a.m > 64 && (a.m + TM - 1) / TM * nblk >= 96;
 }
 
-// How one matrix's k is split over workgroups (a function of the shape alone)
+// How one matrix's k is split over workgroups (a function of the shape alone). Up to 16 rows: only
+// where a wave would have many units. Above, where the column blocks leave CUs without a workgroup
+// (37 x 4096 x 14336: 64 blocks, 25 us with 4 splits, 54 without; two per CU are no better, 31).
 int i4_nsplit(int64_t m, int64_t n, int64_t k, int layout) {
-  if (m > 16) return 1;
-  const int64_t nt = i4_few_tiles(layout, n), blocks = (n + 16 * nt - 1) / (16 * nt);
+  if (m > 64) return 1;
+  const int64_t nt = m > 16 ? 4 : i4_few_tiles(layout, n), blocks = (n + 16 * nt - 1) / (16 * nt);
   const int64_t upw = ((k + 127) / 128 + 7) / 8;  // units per wave of a workgroup
+  if (m > 16) {
+    const int64_t fit = 256 / blocks, s = upw < fit ? upw : fit;
+    return s < 2 ? 1 : (int)(s > 8 ? 8 : s);
+  }
   int64_t s = upw / 4;
   if (s * blocks > 1024) s = 1024 / blocks;
   return upw <= 8 || s < 2 ? 1 : (int)(s > 8 ? 8 : s);
@@ -837,20 +848,34 @@ int i4_launch(const I4Args& a, int nsets, hipStream_t st) {
                        dim3((unsigned)wgs, 1, (unsigned)(SETS == 1 ? nsets : 1)), 512, lds, st, a);
     return check_launch("lcq_int4_gemm");
   }
-  // rows per group decide: up to 16 the smallest tile, above it 64 (32 for two sets) rows a tile
+  // As many row tiles as the rows need. Groups: half as many again as their mean, or most of the
+  // fuller ones would read their weights twice (16 experts of 16 rows, 2048 x 4096: 28 us, 61 with
+  // tiles of 16), and 4 waves instead of 8 (experts of 30 rows, AutoAWQ gate and up: 82 us, 109)
   const int64_t per = a.row_off ? (a.m + a.G - 1) / a.G : a.m;
   constexpr int MB = SETS == 2 ? 2 : 4;
-  const int bm = per <= 16 ? 16 : 16 * MB;
+  const int64_t most = a.row_off ? per + per / 2 : per, tiles = (most + 15) / 16;
+  const int mt = per <= (a.row_off ? 12 : 16) ? 1 : (int)(tiles < MB ? tiles : MB);
+  const int bm = 16 * mt;
   const int64_t slots = a.row_off ? a.m / bm + (a.G < a.m ? a.G : a.m) : (a.m + bm - 1) / bm;
   if (slots > 65535) return fail(LCQ_EINVAL, "lcq_int4_gemm: too many rows");
-  if (per > 16) {
+  if (mt > 1) {
     constexpr int NT = LAYOUT == LA || SETS == 1 ? 4 : 2;
-    return i4_go<DT, LAYOUT, F, MB, NT, SETS, 4>(a, (int)slots, nsets, st);
+    auto go = [&](auto w) {
+      constexpr int W = decltype(w)::value;
+      if constexpr (MB == 4) {
+        if (mt == 4) return i4_go<DT, LAYOUT, F, 4, NT, SETS, W>(a, (int)slots, nsets, st);
+        if (mt == 3) return i4_go<DT, LAYOUT, F, 3, NT, SETS, W>(a, (int)slots, nsets, st);
+      }
+      return i4_go<DT, LAYOUT, F, 2, NT, SETS, W>(a, (int)slots, nsets, st);
+    };
+    if constexpr (SETS == 1)
+      if (!a.row_off) return go(std::integral_constant<int, 8>{});
+    return go(std::integral_constant<int, 4>{});
   }
   if constexpr (LAYOUT == LA || SETS == 2) {
     return i4_go<DT, LAYOUT, F, 1, LAYOUT == LA ? 4 : 2, SETS, 8>(a, (int)slots, nsets, st);
   } else {
-    switch (i4_few_tiles(LAYOUT, a.n)) {
+    switch (i4_few_tiles(LAYOUT, a.row_off ? a.n * (a.G < a.m ? a.G : a.m) : a.n)) {
       case 1: return i4_go<DT, LAYOUT, F, 1, 1, SETS, 8>(a, (int)slots, nsets, st);
       case 2: return i4_go<DT, LAYOUT, F, 1, 2, SETS, 8>(a, (int)slots, nsets, st);
       default: return i4_go<DT, LAYOUT, F, 1, 4, SETS, 8>(a, (int)slots, nsets, st);

@@ -26,6 +26,30 @@ def weight(g, layout, n, k, group, dev):
     return words(k, n // 8), sc(ng, n), words(ng, n // 8)
 
 
+def check_linear(dev, layout, dt, m, n, k, group):
+    from lightcompress_amd import ops
+    g = torch.Generator().manual_seed(m * 7919 + n * 31 + k + group)
+    w = weight(g, layout, n, k, group, dev)
+    x = acts(g, m, k, dt=dt, dev=dev)
+    got = ops.int4_linear(x, *w)
+    assert got.shape == (m, n) and got.dtype == dt
+    y, tol = R.linear(x, *w)
+    assert R.close(got, y, tol)
+    assert torch.equal(got, ops.int4_linear(x, *w))       # the same call, the same bits
+
+
+@pytest.mark.parametrize('layout', ['vllm', 'autoawq'])
+@pytest.mark.parametrize('dt', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('m', [17, 32, 33, 47, 49, 64])
+@pytest.mark.parametrize('n,k,group', [
+    (72, 3200, 128),      # k split 4 ways, the waves' shares of units uneven or empty
+    (264, 9312, 96),      # a last unit that is cut, 32-wide groups of a scale
+    (1288, 2112, 64), (16392, 640, 128)])
+def test_linear_some_rows(dev, layout, dt, m, n, k, group):
+    """17 to 64 rows: two to four row tiles, k split over workgroups where n is small."""
+    check_linear(dev, layout, dt, m, n, k, group)
+
+
 def acts(g, *shape, dt, dev):
     x = torch.randn(*shape, generator=g)
     x[..., :: 37] *= 12          # outlier channels
@@ -136,6 +160,31 @@ def test_grouped(dev, layout, dt, counts, n, k, group):
             assert R.close(one[s], *gu[0])
             assert R.close(two[0, s], *gu[0]) and R.close(two[1, s], *gu[1])
             assert R.close(h[s], *R.silu_mul(*gu))
+
+
+@pytest.mark.parametrize('layout', LAYOUTS)
+@pytest.mark.parametrize('counts,n,k,group', [
+    ([13, 0, 40, 7, 3], 72, 1152, 128),       # a mean of 13 rows: two row tiles
+    ([1, 70, 33, 20], 264, 416, 32), ([48, 49, 1, 17, 50], 520, 640, 64), ([38] * 6, 40, 96, 96),
+    ([47] * 3 + [0], 1032, 2176, 128)])
+def test_grouped_some_rows(dev, layout, counts, n, k, group):
+    """Groups of a few row tiles each."""
+    from lightcompress_amd import ops
+    g = torch.Generator().manual_seed(sum(counts) + n)
+    rows, E = sum(counts), len(counts)
+    off = torch.tensor([0] + counts).cumsum(0)
+    ws = [[weight(g, layout, n, k, group, dev) for _ in range(E)] for _ in range(2)]
+    both = torch.stack([ops.int4_weight_table(w, dev) for w in ws]).contiguous()
+    x = acts(g, rows, k, dt=torch.bfloat16, dev=dev)
+    two = ops.int4_linear_grouped(x, off.to(dev), both, n, group, layout=layout)
+    h = ops.int4_linear_grouped(x, off.to(dev), both, n, group, layout=layout, silu_mul=True)
+    for e in range(E):
+        s = slice(int(off[e]), int(off[e + 1]))
+        if s.start == s.stop:
+            continue
+        gu = [R.linear(x[s], *w[e]) for w in ws]
+        assert R.close(two[0, s], *gu[0]) and R.close(two[1, s], *gu[1])
+        assert R.close(h[s], *R.silu_mul(*gu))
 
 
 @pytest.mark.parametrize('rows', [40, 300])
