@@ -477,14 +477,13 @@ __global__ __launch_bounds__(64 * W) void k_int4_few(I4Args a) {
   }
 }
 
-// Many rows: 128 rows x 256 columns (of one set, or 128 of each of two) per workgroup, 8 waves of
-// 64 x 64. x goes through LDS in units of 128 k (three buffers, one barrier a unit); a wave holds
-// the unit's x fragments (64 registers) and dequantizes its own columns' words, so a word is
-// unpacked once per 64 rows. AutoAWQ words pass through LDS too (transposed reads), vLLM words go
-// straight to registers, and their x is put into the words' element order on its way to LDS. The
-// sums of x of the next unit's groups are formed one unit ahead, one row tile by each wave.
-// What bounds it: per unit and wave 68 MFMAs (1088 cycles) against about 240 (vLLM) / 290
-// (AutoAWQ) vector instructions of 4 cycles, of which half unpack and half scale.
+// Many rows: 128 rows x 256 columns (of one set, or 128 of each of two) per workgroup, 8 waves. x
+// goes through LDS in units of 128 k (three buffers, one barrier a unit); a wave unpacks its
+// columns' words once per unit and walks its row tiles, reading x fragments one tile ahead and
+// scaling a tile's products while the next one's run. vLLM: 128 x 32 a wave, words straight to
+// registers, x put into the words' element order on its way to LDS. AutoAWQ: 64 x 64 a wave, words
+// through LDS too (a transposed read gives 64 columns). The sums of x of the next unit's groups are
+// formed one unit ahead, one row tile by each wave.
 constexpr int TM = 128, TX = TM * 256, TW = 128 * 128;  // rows; bytes of an x, a word buffer
 
 template <int LAYOUT>
@@ -493,11 +492,13 @@ constexpr int i4_tile_lds = 3 * TX + (LAYOUT == LA ? 3 * TW : 0) + 2 * 4 * TM * 
 template <int DT, int LAYOUT, int F, int SETS>
 __global__ __launch_bounds__(512, 2) void k_int4_tile(I4Args a) {
   extern __shared__ __attribute__((aligned(1024))) char i4_lds[];
-  constexpr int NC = SETS == 2 ? 32 : 64;        // columns of a set per wave
+  constexpr int MI = LAYOUT == LV ? 8 : 4, NI = LAYOUT == LV ? 2 : 4;  // 16 x 16 tiles of a wave
+  constexpr int NC = 16 * NI / SETS, WC = 256 / SETS;  // columns of a set per wave, workgroup
   constexpr int NX = LAYOUT == LA ? 3 * TW : 0;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c = lane & 15, q = lane >> 4, mh = w >> 2, nw = w & 3;
-  const int nblk = (int)((a.n + 4 * NC - 1) / (4 * NC));
+  const int c = lane & 15, q = lane >> 4;
+  const int mh = LAYOUT == LV ? 0 : w >> 2, nw = LAYOUT == LV ? w : w & 3;
+  const int nblk = (int)((a.n + WC - 1) / WC);
   // neighbouring workgroups share their weights (one matrix) or their rows (grouped)
   const int id = i4_block(blockIdx.x, gridDim.x);
   int64_t r0, r1;
@@ -515,7 +516,7 @@ __global__ __launch_bounds__(512, 2) void k_int4_tile(I4Args a) {
   const uint16_t* sc[SETS];
   const uint32_t* qz[SETS];
   i4_weights<SETS>(a, grp, qw, sc, qz);
-  const int64_t n0 = (int64_t)nbk * 4 * NC + nw * NC;  // this wave's first column of a set
+  const int64_t n0 = (int64_t)nbk * WC + nw * NC;  // this wave's first column of a set
   const int k = (int)a.k, nb = (k + 127) / 128;
   const uint32_t lds0 = lds_addr(i4_lds), xs0 = lds0 + 3 * TX + NX;
 
@@ -550,7 +551,7 @@ __global__ __launch_bounds__(512, 2) void k_int4_tile(I4Args a) {
   if constexpr (LAYOUT == LA) {
     // a wave's instruction i fills rows 16 w + 8 i .. + 7; this lane's chunk of row lane / 8
     const int r = lane >> 3, ch = (lane & 7) ^ (((r >> 1) & 3) << 1);
-    const int64_t at = (int64_t)nbk * 2 * NC;
+    const int64_t at = (int64_t)nbk * (WC / 2);
     const int64_t byte = SETS == 2 ? at + 16 * (ch >> 1) : at + 16 * ch;
     wsrc = reinterpret_cast<uint64_t>(qw[SETS == 2 ? ch & 1 : 0]) + min(byte, a.n / 2 - 16);
   }
@@ -566,43 +567,44 @@ __global__ __launch_bounds__(512, 2) void k_int4_tile(I4Args a) {
       dma16_at(wbuf + 1024 * (2 * w + i),
                wsrc + (uint64_t)min(128 * u + 16 * w + 8 * i + (lane >> 3), k - 1) * ldw);
   };
-  // vLLM words and the scales of a unit
-  uint32_t wo[4];
-  uint32_t so, zo = 0;
-  const char* sp;
+  // vLLM words and the scales of a unit; column tile t of vLLM is set t / (2 / SETS)
+  uint32_t wo[NI], so[LAYOUT == LV ? NI : 1], zo = 0;
+  const char* sp = nullptr;
   const char* zp = nullptr;
   const uint32_t lds_s = LAYOUT == LV ? (uint32_t)(a.k / a.group * 2) : (uint32_t)(a.n * 2);
   if constexpr (LAYOUT == LV) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-      wo[t] = (uint32_t)min(n0 + 16 * (SETS == 2 ? t & 1 : t) + c, a.n - 1) * (uint32_t)(k / 2);
-    so = (uint32_t)min(n0 + 16 * (SETS == 2 ? q & 1 : q) + c, a.n - 1) * lds_s;  // tile q's scale
-    sp = reinterpret_cast<const char*>(sc[SETS == 2 ? q >> 1 : 0]);
+    for (int t = 0; t < NI; ++t) {
+      const uint32_t row = (uint32_t)min(n0 + 16 * (SETS == 2 ? 0 : t) + c, a.n - 1);
+      wo[t] = row * (uint32_t)(k / 2);
+      so[t] = row * lds_s;
+    }
   } else {
     const int s = SETS == 2 ? c >> 3 : 0;
     const uint32_t wc = (uint32_t)min(n0 / 8 + ((SETS == 2 ? c & 7 : c) >> 1), a.n / 8 - 1);
-    so = 16 * wc;
+    so[0] = 16 * wc;
     zo = 4 * wc;
     sp = reinterpret_cast<const char*>(sc[s]);
     zp = reinterpret_cast<const char*>(qz[s]);
   }
-  i4_v4u wv[LAYOUT == LV ? 4 : 1];
-  uint32_t sv4[F][LAYOUT == LV ? 1 : 4], zv1[LAYOUT == LV ? 1 : F];
+  i4_v4u wv[LAYOUT == LV ? NI : 1];
+  uint32_t sv4[F][LAYOUT == LV ? NI : 4], zv1[LAYOUT == LV ? 1 : F];
   auto w_load = [&](int u) {
     const int k0 = 128 * u;
     if constexpr (LAYOUT == LV) {
       const uint32_t kw = (uint32_t)min(k0 + 32 * q, k - 32) / 2;
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-        wv[t] = gload<i4_v4u>(qw[SETS == 2 ? t >> 1 : 0], wo[t] + kw);
+      for (int t = 0; t < NI; ++t) wv[t] = gload<i4_v4u>(qw[SETS == 2 ? t : 0], wo[t] + kw);
     }
 #pragma unroll
     for (int f = 0; f < F; ++f) {
       const uint32_t gi = i4_group(a, (uint32_t)min(k0 + 128 / F * f, k - 32));
       if constexpr (LAYOUT == LV) {
-        sv4[f][0] = gload<uint16_t>(sp, so + 2 * gi);
+#pragma unroll
+        for (int t = 0; t < NI; ++t)
+          sv4[f][t] = gload<uint16_t>(sc[SETS == 2 ? t : 0], so[t] + 2 * gi);
       } else {
-        const i4_v4u v = gload<i4_v4u>(sp, so + gi * lds_s);
+        const i4_v4u v = gload<i4_v4u>(sp, so[0] + gi * lds_s);
 #pragma unroll
         for (int j = 0; j < 4; ++j) sv4[f][j] = v[j];
         zv1[f] = gload<uint32_t>(zp, zo + gi * ldw);
@@ -610,32 +612,34 @@ __global__ __launch_bounds__(512, 2) void k_int4_tile(I4Args a) {
     }
   };
   // x fragment of row tile i, k-step j. vLLM with F 1: word j of lane q holds k = 32 q + 8 j
-  auto x_frag = [&](uint32_t buf, int i, int j) {
-    const int ch = LAYOUT == LV && F == 1 ? 4 * q + j : 4 * j + q;
-    return __builtin_bit_cast(i4_v4u, lds_read16(buf + 4096 * i + 256 * c + 16 * (ch ^ i4_swz(c))));
-  };
+  uint32_t xo[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    xo[j] = 256 * c + 16 * ((LAYOUT == LV && F == 1 ? 4 * q + j : 4 * j + q) ^ i4_swz(c));
   const i4_v4f zero = {0.f, 0.f, 0.f, 0.f};
   const i4_v4u ones = {i4_ones<DT>, i4_ones<DT>, i4_ones<DT>, i4_ones<DT>};
   const I4Const<DT> kc;
-  auto x_sums = [&](int u, uint32_t buf) {  // of row tile 4 mh + nw, to the unit's sum buffer
+  // sums of row tile w, to the unit's sum buffer (vLLM: times -(16 + z), z = 8)
+  auto x_sums = [&](int u, uint32_t buf) {
 #pragma unroll
     for (int f = 0; f < F; ++f) {
       i4_v4f xs = zero;
 #pragma unroll
       for (int j = 4 / F * f; j < 4 / F * (f + 1); ++j)
         if (F == 1 || 128 * u + 32 * j < k)
-          xs = i4_mfma<DT>(x_frag(buf, 4 * mh + nw, j), ones, xs);
+          xs = i4_mfma<DT>(__builtin_bit_cast(i4_v4u, lds_read16(buf + 4096 * w + xo[j])), ones, xs);
+      if constexpr (LAYOUT == LV) xs *= -24.f;
       if (c == 0)
         *reinterpret_cast<i4_v4f*>(i4_lds + (xs0 - lds0) + ((u & 1) * 4 + f) * TM * 4 +
-                                   (16 * (4 * mh + nw) + 4 * q) * 4) = xs;
+                                   (16 * w + 4 * q) * 4) = xs;
     }
   };
 
-  i4_v4f acc[4][4];
+  i4_v4f acc[MI][NI];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) acc[i][t] = zero;
+    for (int t = 0; t < NI; ++t) acc[i][t] = zero;
 
   uint32_t xb[3] = {lds0, lds0 + TX, lds0 + 2 * TX};
   uint32_t wb[3] = {lds0 + 3 * TX, lds0 + 3 * TX + TW, lds0 + 3 * TX + 2 * TW};
@@ -661,14 +665,14 @@ __global__ __launch_bounds__(512, 2) void k_int4_tile(I4Args a) {
     // the next unit's x (and words) and this one's sums are in LDS; the oldest buffer is free
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    i4_v4u wc4[LAYOUT == LV ? 4 : 1];
-    uint32_t sc4[F][LAYOUT == LV ? 1 : 4], zc1[LAYOUT == LV ? 1 : F];
+    i4_v4u wc4[LAYOUT == LV ? NI : 1];
+    uint32_t sc4[F][LAYOUT == LV ? NI : 4], zc1[LAYOUT == LV ? 1 : F];
 #pragma unroll
-    for (int t = 0; t < (LAYOUT == LV ? 4 : 0); ++t) wc4[t] = F == 1 ? wv[t] : i4_transpose(wv[t]);
+    for (int t = 0; t < (LAYOUT == LV ? NI : 0); ++t) wc4[t] = F == 1 ? wv[t] : i4_transpose(wv[t]);
 #pragma unroll
     for (int f = 0; f < F; ++f) {
 #pragma unroll
-      for (int j = 0; j < (LAYOUT == LV ? 1 : 4); ++j) sc4[f][j] = sv4[f][j];
+      for (int j = 0; j < NI; ++j) sc4[f][j] = sv4[f][j];
       if constexpr (LAYOUT == LA) zc1[f] = zv1[f];
     }
     if constexpr (LAYOUT == LA) {
@@ -682,56 +686,67 @@ __global__ __launch_bounds__(512, 2) void k_int4_tile(I4Args a) {
       if (u + 1 < nb) w_load(u + 1);
     }
     if (u + 1 < nb) x_sums(u + 1, xb[1]);
-    i4_v4u xf[4][4];
+    constexpr int J = 4 / F;
+    i4_v4u xf[2][J];
+    i4_v4f xs[2], g[2][NI];
+    const uint32_t xbase = xb[0] + 16384 * mh, sbase = xs0 + (u & 1) * 4 * TM * 4 + 256 * mh + 16 * q;
+    auto fetch = [&](int f, int i) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) xf[i][j] = x_frag(xb[0] + 16384 * mh, i, j);
+      for (int j = 0; j < J; ++j)
+        xf[i & 1][j] = __builtin_bit_cast(i4_v4u, lds_read16(xbase + xo[J * f + j] + 4096 * i));
+      xs[i & 1] = __builtin_bit_cast(i4_v4f, lds_read16(sbase + f * TM * 4 + 64 * i));
+    };
 #pragma unroll
     for (int f = 0; f < F; ++f) {
       if (F > 1 && 128 * u + 128 / F * f >= k) break;
-      i4_v4f xs[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        xs[i] = *reinterpret_cast<const i4_v4f*>(
-            i4_lds + (xs0 - lds0) + ((u & 1) * 4 + f) * TM * 4 + (64 * mh + 16 * i + 4 * q) * 4);
-        if constexpr (LAYOUT == LV) xs[i] *= -24.f;
-      }
-      i4_v4u pk[LAYOUT == LA ? 4 / F : 1];
+      fetch(f, 0);
+      i4_v4u bf[NI][J];
+      float s[NI], z[NI];
       if constexpr (LAYOUT == LA) {
         typedef uint32_t v2u_t __attribute__((ext_vector_type(2)));
 #pragma unroll
-        for (int j = 0; j < 4 / F; ++j) {
-          const uint32_t at = wb[0] + 4096 * (4 / F * f + j);
+        for (int j = 0; j < J; ++j) {
+          const uint32_t at = wb[0] + 4096 * (J * f + j);
           const v2u_t l = __builtin_bit_cast(v2u_t, lds_read_tr(at + trl));
           const v2u_t h = __builtin_bit_cast(v2u_t, lds_read_tr(at + trh));
-          pk[j] = i4_v4u{l.x, l.y, h.x, h.y};
+          const i4_v4u pk = {l.x, l.y, h.x, h.y};
+#pragma unroll
+          for (int t = 0; t < NI; ++t) bf[t][j] = i4_nibble<DT>(pk, t, kc);
         }
       }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        float s, z;
+      for (int t = 0; t < NI; ++t) {
         if constexpr (LAYOUT == LV) {
-          s = h2f((uint16_t)__shfl(sc4[f][0], 16 * t + c));
-          z = 0.f;
+          s[t] = h2f((uint16_t)sc4[f][t]);
+          z[t] = 0.f;
+#pragma unroll
+          for (int j = 0; j < J; ++j) bf[t][j] = i4_word<DT>(wc4[LAYOUT == LV ? t : 0][J * f + j], kc);
         } else {
-          s = h2f((uint16_t)(sc4[f][t] >> (c & 1 ? 16 : 0)));
-          z = 16.f + (float)((zc1[f] >> (4 * t + 16 * (c & 1))) & 15u);
+          s[t] = h2f((uint16_t)(sc4[f][t] >> (c & 1 ? 16 : 0)));
+          z[t] = -16.f - (float)((zc1[f] >> (4 * t + 16 * (c & 1))) & 15u);
         }
-        i4_v4f g[4];
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) g[i] = LAYOUT == LV ? xs[i] : -z * xs[i];
+      for (int i = 0; i <= MI; ++i) {
+        if (i + 1 < MI) fetch(f, i + 1);
+        if (i < MI) {
 #pragma unroll
-        for (int j = 0; j < 4 / F; ++j) {
-          const i4_v4u bf = LAYOUT == LV ? i4_word<DT>(wc4[LAYOUT == LV ? t : 0][4 / F * f + j], kc)
-                                         : i4_nibble<DT>(pk[LAYOUT == LA ? j : 0], t, kc);
+          for (int t = 0; t < NI; ++t)
+            g[i & 1][t] = LAYOUT == LV ? xs[i & 1] : z[t] * xs[i & 1];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) g[i] = i4_mfma<DT>(xf[i][4 / F * f + j], bf, g[i]);
+          for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int t = 0; t < NI; ++t)
+              g[i & 1][t] = i4_mfma<DT>(xf[i & 1][j], bf[t][j], g[i & 1][t]);
         }
+        if (i > 0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+          for (int t = 0; t < NI; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][t][r] = __fmaf_rn(s, g[i][r], acc[i][t][r]);
+            for (int r = 0; r < 4; ++r)
+              acc[i - 1][t][r] = __fmaf_rn(s[t], g[(i - 1) & 1][t][r], acc[i - 1][t][r]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     if constexpr (LAYOUT == LA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -740,35 +755,36 @@ __global__ __launch_bounds__(512, 2) void k_int4_tile(I4Args a) {
     wb[0] = wb[1]; wb[1] = wb[2]; wb[2] = w0;
   }
   __syncthreads();
-  // the wave's tile through LDS (its own 8 KB, rows of 64 columns of 2 bytes) to row-wise stores
+  // the wave's tile through LDS (its own 8 KB) to row-wise stores; chunks of 8 columns swizzled by
+  // the row: 16 rows of a column spread over the banks
+  constexpr int RB = 32 * NI, SW = RB / 16 - 1;  // bytes of a row, chunks - 1
   char* out = i4_lds + 8192 * w;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int row = 16 * i + 4 * q + r;
 #pragma unroll
-      for (int t = 0; t < (SETS == 2 && LAYOUT == LV ? 2 : 4); ++t) {
+      for (int t = 0; t < (LAYOUT == LV ? NI / SETS : NI); ++t) {
         float o = acc[i][t][r];
-        int col = LAYOUT == LV ? 16 * t + c : i4_awq_column(c, t);
+        const int col = LAYOUT == LV ? 16 * t + c : i4_awq_column(c, t);
         if constexpr (SETS == 2) {
-          const float up = LAYOUT == LV ? acc[i][t + 2][r] : __shfl_xor(o, 8);
+          const float up = LAYOUT == LV ? acc[i][1][r] : __shfl_xor(o, 8);
           o = o / (1.f + expf(-o)) * up;
         }
         if (a.bias) o += ld1<DT>(a.bias, min(n0 + col, a.n - 1));
-        // chunks of 8 columns swizzled by the row: 16 rows of a column spread over the banks
         if (SETS == 1 || LAYOUT == LV || c < 8)
-          st1<DT>(out + 128 * row + 16 * ((col >> 3) ^ (row & 7)), col & 7, o);
+          st1<DT>(out + RB * row + 16 * ((col >> 3) ^ (row & SW)), col & 7, o);
       }
     }
   __syncthreads();
   constexpr int CPR = NC / 8;  // 16-byte chunks of a row
 #pragma unroll
-  for (int e = 0; e < CPR; ++e) {
+  for (int e = 0; e < MI * CPR / 4; ++e) {
     const int row = e * (64 / CPR) + lane / CPR, ch = lane % CPR;
     const int64_t gr = r0 + 64 * mh + row, col = n0 + 8 * ch;
     if (gr >= r1) continue;
-    i4_v4u v = *reinterpret_cast<const i4_v4u*>(out + 128 * row + 16 * (ch ^ (row & 7)));
+    i4_v4u v = *reinterpret_cast<const i4_v4u*>(out + RB * row + 16 * (ch ^ (row & SW)));
     if (a.a_rows && (a.a_rows[gr] < 0 || a.a_rows[gr] >= a.x_rows)) v = i4_v4u{0, 0, 0, 0};
     uint16_t* yp = a.y + (a.row_off && SETS == 1 ? blockIdx.z * a.m * a.ldy : 0) + gr * a.ldy + col;
     if (a.wide_y && col + 8 <= a.n) {
