@@ -689,12 +689,20 @@ __global__ __launch_bounds__(512, 2) void k_int4_tile(I4Args a) {
     constexpr int J = 4 / F;
     i4_v4u xf[2][J];
     i4_v4f xs[2], g[2][NI];
-    const uint32_t xbase = xb[0] + 16384 * mh, sbase = xs0 + (u & 1) * 4 * TM * 4 + 256 * mh + 16 * q;
+    // (the empty asm keeps a lane's addresses whole, so that tiles and groups are read at constant
+    // offsets: the compiler would add up each address instead)
+    uint32_t xa[4], sa = xs0 + (u & 1) * 4 * TM * 4 + 256 * mh + 16 * q;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      xa[j] = xb[0] + 16384 * mh + xo[j];
+      asm volatile("" : "+v"(xa[j]));
+    }
+    asm volatile("" : "+v"(sa));
     auto fetch = [&](int f, int i) {
 #pragma unroll
       for (int j = 0; j < J; ++j)
-        xf[i & 1][j] = __builtin_bit_cast(i4_v4u, lds_read16(xbase + xo[J * f + j] + 4096 * i));
-      xs[i & 1] = __builtin_bit_cast(i4_v4f, lds_read16(sbase + f * TM * 4 + 64 * i));
+        xf[i & 1][j] = __builtin_bit_cast(i4_v4u, lds_read16(xa[J * f + j] + 4096 * i));
+      xs[i & 1] = __builtin_bit_cast(i4_v4f, lds_read16(sa + f * TM * 4 + 64 * i));
     };
 #pragma unroll
     for (int f = 0; f < F; ++f) {
@@ -817,20 +825,18 @@ bool i4_use_tile(const I4Args& a, int layout, int sets) {
   return a.m > 64 && (a.m + TM - 1) / TM * nblk >= 96;
 }
 
-// How one matrix's k is split over workgroups (a function of the shape alone). Up to 16 rows: only
-// where a wave would have many units. Above, where the column blocks leave CUs without a workgroup
-// (37 x 4096 x 14336: 64 blocks, 25 us with 4 splits, 54 without; two per CU are no better, 31).
+// How one matrix's k is split over workgroups (a function of the shape alone): where the column
+// blocks leave CUs without a workgroup, and up to 16 rows only where the waves have units enough to
+// pay for the join. 1 x 4096 x 14336 AutoAWQ, 64 blocks: 16.5 us with 4 splits, 28.9 without, 17.6
+// with 8; at k 4096 8.9 with 2, 7.7 without. 37 x 4096 x 14336: 25 us with 4, 54 without, 31 with 8.
 int i4_nsplit(int64_t m, int64_t n, int64_t k, int layout) {
   if (m > 64) return 1;
   const int64_t nt = m > 16 ? 4 : i4_few_tiles(layout, n), blocks = (n + 16 * nt - 1) / (16 * nt);
   const int64_t upw = ((k + 127) / 128 + 7) / 8;  // units per wave of a workgroup
-  if (m > 16) {
-    const int64_t fit = 256 / blocks, s = upw < fit ? upw : fit;
-    return s < 2 ? 1 : (int)(s > 8 ? 8 : s);
-  }
-  int64_t s = upw / 4;
-  if (s * blocks > 1024) s = 1024 / blocks;
-  return upw <= 8 || s < 2 ? 1 : (int)(s > 8 ? 8 : s);
+  if (m <= 16 && upw <= (layout == LA ? 6 : 8)) return 1;
+  const int64_t most = m > 16 ? upw : upw / 2, fit = 256 / blocks;
+  const int64_t s = most < fit ? most : fit;
+  return s < 2 ? 1 : (int)(s > 8 ? 8 : s);
 }
 
 template <int DT, int LAYOUT, int F, int MT, int NT, int SETS, int W>
