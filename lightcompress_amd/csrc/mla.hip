@@ -49,7 +49,7 @@ __device__ __forceinline__ int64_t uni(int64_t v) {
 constexpr int FQT = 128;  // query rows per workgroup (4 waves of 32)
 constexpr int FKT = 64;   // keys per tile
 constexpr int F_STAGE = FKT * (DN + DR + DV) * 2;  // 40 KB
-constexpr int F_AHEAD = 6;                         // LDS fragments read ahead of their product
+constexpr int F_AHEAD = 4;                         // LDS fragments read ahead of their product
 constexpr int F_MIN = 8;                           // least tiles of a share of the keys
 constexpr int F_PART = FQT * DV;                   // floats of a query tile's partial output
 
@@ -71,29 +71,32 @@ struct MlaFwdArgs {
 // sequence is never loaded.
 struct FwdStage {
   uint32_t kn[4], v[4], kr[2];
-  __device__ __forceinline__ void init(const MlaFwdArgs& a, int lim, int w, int lane) {
+  __device__ __forceinline__ void init_keys(const MlaFwdArgs& a, int lim, int w, int lane) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = 4 * (4 * w + j) + (lane >> 4);
-      const uint32_t ch = 16 * ((lane & 15) ^ swz16(row)), key = min(row, lim);
-      kn[j] = key * (uint32_t)a.kns * 2 + ch;
-      v[j] = key * (uint32_t)a.vs * 2 + ch;
-    }
+    for (int j = 0; j < 4; ++j) kn[j] = at(4 * (4 * w + j) + (lane >> 4), lim, a.kns, lane);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int row = 8 * (2 * w + j) + (lane >> 3);
       kr[j] = (uint32_t)min(row, lim) * (uint32_t)a.krs * 2 + 16 * ((lane & 7) ^ ((row >> 1) & 7));
     }
   }
-  __device__ __forceinline__ void issue(uint32_t st, const uint16_t* pn, const uint16_t* pr,
-                                        const uint16_t* pv, int w) const {
+  __device__ __forceinline__ void init_values(const MlaFwdArgs& a, int lim, int w, int lane) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      dma16(st + 1024 * (4 * w + j), pn, kn[j]);
-      dma16(st + 16384 + 1024 * (4 * w + j), pv, v[j]);
-    }
+    for (int j = 0; j < 4; ++j) v[j] = at(4 * (4 * w + j) + (lane >> 4), lim, a.vs, lane);
+  }
+  static __device__ __forceinline__ uint32_t at(int row, int lim, int64_t stride, int lane) {
+    return (uint32_t)min(row, lim) * (uint32_t)stride * 2 + 16 * ((lane & 15) ^ swz16(row));
+  }
+  __device__ __forceinline__ void keys(uint32_t st, const uint16_t* pn, const uint16_t* pr,
+                                       int w) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dma16(st + 1024 * (4 * w + j), pn, kn[j]);
 #pragma unroll
     for (int j = 0; j < 2; ++j) dma16(st + 32768 + 1024 * (2 * w + j), pr, kr[j]);
+  }
+  __device__ __forceinline__ void values(uint32_t st, const uint16_t* pv, int w) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dma16(st + 16384 + 1024 * (4 * w + j), pv, v[j]);
   }
 };
 
@@ -146,13 +149,22 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
   const uint16_t* krp = uni(a.kr + b * a.krb);
   const uint16_t* vp = uni(a.v + b * a.vb + hq * a.vh);
   FwdStage fs;
-  fs.init(a, min(FKT - 1, klen - 1 - kbeg), w, lane);
-  auto stage = [&](int k0, int buf) {  // called for tile after tile
-    if (k0 > kbeg && klen - 1 - k0 < FKT - 1) fs.init(a, klen - 1 - k0, w, lane);
-    fs.issue(lds0 + buf * F_STAGE, uni(knp + k0 * a.kns), uni(krp + k0 * a.krs),
-             uni(vp + k0 * a.vs), w);
+  const int lim0 = min(FKT - 1, klen - 1 - kbeg);
+  fs.init_keys(a, lim0, w, lane);
+  fs.init_values(a, lim0, w, lane);
+  const int ntile = (kend - kbeg + FKT - 1) / FKT;
+  // called for tile after tile; keys and values have two buffers each
+  auto stage_keys = [&](int t) {
+    const int k0 = kbeg + t * FKT;
+    if (t > 0 && klen - 1 - k0 < FKT - 1) fs.init_keys(a, klen - 1 - k0, w, lane);
+    fs.keys(lds0 + (t & 1) * F_STAGE, uni(knp + k0 * a.kns), uni(krp + k0 * a.krs), w);
   };
-  stage(kbeg, 0);
+  auto stage_values = [&](int t) {
+    const int k0 = kbeg + t * FKT;
+    if (t > 0 && klen - 1 - k0 < FKT - 1) fs.init_values(a, klen - 1 - k0, w, lane);
+    fs.values(lds0 + (t & 1) * F_STAGE, uni(vp + k0 * a.vs), w);
+  };
+  stage_keys(0);
 
   const int qrow = q0 + 32 * w + c;  // this lane's query row (both halves)
   // Q^T as the B operand of mfma(K, Q^T): lane holds Q[qrow][16 kk + 8 h + j]
@@ -182,40 +194,41 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
   const uint32_t va = 16384 + 256 * (4 * (g >> 1) + qq) +
                       16 * ((2 * (g & 1) + (pp >> 1)) ^ (qq << 2 | (g >> 1))) + 8 * (pp & 1);
 
-  int it = 0;
-  for (int k0 = kbeg; k0 < kend; k0 += FKT, ++it) {
-    const uint32_t cur = lds0 + (it & 1) * F_STAGE;
-    // this wave's part of the tile has arrived; behind the barrier every wave's has, and every
-    // wave is done with the tile before, whose stage is filled next
+  // one product of S^T = K Q^T (two tiles of 32 keys in turn, so that a product does not wait for
+  // the one before it): product f is k-step f / 2 of tile f & 1. Register r of tile t holds key
+  // 32 t + (r & 3) + 8 (r >> 2) + 4 h of the lane's row
+  auto kfrag = [&](uint32_t st, int f) {
+    const int kk = f >> 1, t = f & 1;
+    return kk < 8 ? lds_read16(((st + ka) ^ (32 * kk)) + 8192 * t)
+                  : lds_read16(((st + ra) ^ (32 * (kk - 8))) + 4096 * t);
+  };
+  v16f_t s[2];
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  if (ntile > 1) stage_keys(1);
+  stage_values(0);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.f;
+  if (kbeg <= wmax) {
+#pragma unroll
+    for (int f = 0; f < 24; ++f) s[f & 1] = mfma32<DT>(kfrag(lds0, f), qf[f >> 1], s[f & 1]);
+  }
+
+  // Iteration t: the softmax of tile t's scores stands between the products of tile t + 1's (the
+  // matrix pipe and the vector pipe work at once), then O^T += V^T P^T. K fragments are read
+  // F_AHEAD products ahead (the scheduling barriers keep the compiler to that order: left alone
+  // it waits for each read right before its product)
+  for (int it = 0; it < ntile; ++it) {
+    const int k0 = kbeg + it * FKT;
+    const uint32_t cur = lds0 + (it & 1) * F_STAGE, nxt = lds0 + ((it & 1) ^ 1) * F_STAGE;
+    // this wave's part of K(t + 1) and V(t) has arrived; behind the barrier every wave's has, and
+    // every wave is done with K(t) and V(t - 1), whose buffers are filled next
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    if (k0 + FKT < kend) stage(k0 + FKT, (it & 1) ^ 1);
-    if (k0 > wmax) continue;  // no row of this wave sees the tile
+    if (it + 2 < ntile) stage_keys(it + 2);
+    if (it + 1 < ntile) stage_values(it + 1);
+    if (k0 > wmax) continue;  // no row of this wave sees the tile, nor a later one
 
-    // S^T tiles t: register r holds key k0 + 32 t + (r & 3) + 8 (r >> 2) + 4 h of the lane's row.
-    // The two tiles in turn, so that a product does not wait for the one before it; K fragments
-    // are read F_AHEAD products ahead (the scheduling barriers keep the compiler to that order:
-    // left alone it waits for each read right before its product)
-    v16f_t s[2];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.f;
-    {
-      const uint32_t kb = cur + ka, rp = cur + ra;
-      auto kfrag = [&](int f) {  // product f: k-step f / 2 of tile f & 1
-        const int kk = f >> 1, t = f & 1;
-        return kk < 8 ? lds_read16((kb ^ (32 * kk)) + 8192 * t)
-                      : lds_read16((rp ^ (32 * (kk - 8))) + 4096 * t);
-      };
-      v8s_t kf[F_AHEAD];
-#pragma unroll
-      for (int f = 0; f < F_AHEAD; ++f) kf[f] = kfrag(f);
-#pragma unroll
-      for (int f = 0; f < 24; ++f) {
-        s[f & 1] = mfma32<DT>(kf[f % F_AHEAD], qf[f >> 1], s[f & 1]);
-        if (f + F_AHEAD < 24) kf[f % F_AHEAD] = kfrag(f + F_AHEAD);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
     if (k0 + FKT - 1 > wmin) {  // wave-uniform: some key is hidden from some row
       const int lim = pos - k0 - 4 * h;
 #pragma unroll
@@ -244,26 +257,37 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
     }
     const float msub = m == -INFINITY ? 0.f : m;
     float rs = 0.f;
+    v8s_t pf[4];  // k-step ts = (t, s2) of P^T: score registers 8 s2 .. 8 s2 + 7 of tile t
+    auto soft = [&](int e, float msub) {  // weights 2 e, 2 e + 1 of 32
+      const int t = e >> 3, r = 2 * (e & 7);
+      const float p0 = __builtin_amdgcn_exp2f(__fmaf_rn(s[t][r], a.sl2, -msub));
+      const float p1 = __builtin_amdgcn_exp2f(__fmaf_rn(s[t][r + 1], a.sl2, -msub));
+      rs += p0;
+      rs += p1;
+      reinterpret_cast<uint32_t*>(&pf[2 * t + (r >> 3)])[(r & 7) >> 1] = pack_dt<DT>(p0, p1);
+    };
+    v16f_t n[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int r = 0; r < 16; ++r) n[0][r] = n[1][r] = 0.f;
+    if (it + 1 < ntile) {
+      float ms = msub;  // its own value, or the compiler would lift the weights above the branch
+      asm volatile("" : "+v"(ms));
+      v8s_t kf[F_AHEAD];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float p = __builtin_amdgcn_exp2f(__fmaf_rn(s[t][r], a.sl2, -msub));
-        s[t][r] = p;
-        rs += p;
+      for (int f = 0; f < F_AHEAD; ++f) kf[f] = kfrag(nxt, f);
+#pragma unroll
+      for (int f = 0; f < 24; ++f) {
+        n[f & 1] = mfma32<DT>(kf[f % F_AHEAD], qf[f >> 1], n[f & 1]);
+        if (f + F_AHEAD < 24) kf[f % F_AHEAD] = kfrag(nxt, f + F_AHEAD);
+        if (f >= 3 && f < 19) soft(f - 3, ms);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    l += rs + other_half(rs, h);
-    // O^T += V^T P^T; k-step ts = (t, s2): score registers 8 s2 .. 8 s2 + 7 of tile t, V^T fragments
-    // by transposed reads of the same keys' rows
-    v8s_t pf[4];
+    } else {
 #pragma unroll
-    for (int ts = 0; ts < 4; ++ts) {
-      uint32_t* pw = reinterpret_cast<uint32_t*>(&pf[ts]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        pw[j] = pack_dt<DT>(s[ts >> 1][8 * (ts & 1) + 2 * j], s[ts >> 1][8 * (ts & 1) + 2 * j + 1]);
+      for (int e = 0; e < 16; ++e) soft(e, msub);
     }
-    {
+    l += rs + other_half(rs, h);
+    {  // V^T fragments by transposed reads of the keys' rows
       const uint32_t vb = cur + va;
       auto vfrag = [&](int f) {  // product f: k-step f / 4, dims 32 (f & 3) ..
         const uint32_t at = (vb ^ (64 * (f & 3))) + 4096 * (f >> 2);
@@ -280,6 +304,8 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    s[0] = n[0];
+    s[1] = n[1];
   }
   if constexpr (SPLIT) {
     float4* dst = reinterpret_cast<float4*>(a.part + pt * F_PART) + tid;
