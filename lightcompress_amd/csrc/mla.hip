@@ -431,7 +431,7 @@ constexpr int D_RING = 8;                        // tiles whose key addresses ar
 constexpr int dec_tab(int nst) { return nst == 4 ? 64 : 16; }
 constexpr int D_ROWS = 16;                       // query rows (token x head) per wave
 constexpr int D_PART = D_ROWS * DL;              // floats of one row block's partial output
-constexpr int D_MIN = 2;                         // least tiles of a workgroup
+constexpr int D_CUTS = 48;                       // most partial outputs of a line of tiles, on average
 constexpr int D_AHEAD = 4;                       // LDS fragments read ahead of their product
 
 typedef float v4f_t __attribute__((ext_vector_type(4)));
@@ -485,7 +485,7 @@ struct MlaDecArgs {
 // ---- how the work is divided -----------------------------------------------------------
 // A sequence b takes n_b = max(1, ceil(len / 32)) key tiles, once for each of its ny groups of RB row
 // blocks. The tiles of all (b, group) stand in one line, b major, and the line is cut into wgs
-// equal ranges (fewer where a range would fall below D_MIN tiles), one workgroup each: whatever
+// equal ranges, one workgroup each: whatever
 // the lengths, the workgroups do the same work. A (b, group) inside one range is finished by its
 // workgroup; one that a cut divides leaves partial outputs in its workgroups' slots, 2 i for the
 // segment that workgroup i begins with, 2 i + 1 for another one, and k_mla_join adds them in order.
@@ -530,7 +530,7 @@ __device__ __forceinline__ int dec_find(const MlaDecArgs& a, int at, int& first)
 }
 // tiles of a range
 __device__ __forceinline__ int dec_step(const MlaDecArgs& a, int total) {
-  return max(D_MIN, (total + a.wgs - 1) / a.wgs);
+  return (total + a.wgs - 1) / a.wgs;
 }
 
 // One wave per 16 query rows, RB waves per workgroup sharing the key tiles. Scores are held
@@ -774,11 +774,13 @@ __global__ void __launch_bounds__(64 * RB, 2) k_mla_dec(MlaDecArgs a) {
   }
 }
 
-// Joins the partial outputs of one row block in key order: 8 workgroups of 256 threads per block, a
-// thread one float4 (4 dims of a row) of every partial.
-template <int DT, int RB>
+// Joins the partial outputs of one row block in key order. A thread takes one float4 (4 dims of a
+// row) of every partial (W 1: 8 workgroups per block), or of a quarter of them, the workgroup's
+// four waves one after the other in the end (W 4: 32 workgroups per block, for many partials).
+template <int DT, int RB, int W>
 __global__ void __launch_bounds__(256) k_mla_join(MlaDecArgs a) {
-  const int b = blockIdx.y, rb = blockIdx.x >> 3;
+  __shared__ float red[W == 1 ? 1 : 3][64][6];
+  const int b = blockIdx.y, rb = blockIdx.x / (8 * W), wave = threadIdx.x >> 6;
   const int y = rb / RB, w = rb - y * RB;
   const int total = dec_total(a), step = dec_step(a, total);
   int s = 0;
@@ -793,36 +795,55 @@ __global__ void __launch_bounds__(256) k_mla_join(MlaDecArgs a) {
   s = __builtin_amdgcn_readfirstlane(s) + y * nt;          // this block's first tile
   const int i0 = s / step, i1 = (s + nt - 1) / step;       // the workgroups that hold its tiles
   if (i0 == i1) return;                                    // finished by its workgroup
-  const int at4 = (blockIdx.x & 7) * 256 + threadIdx.x;  // float4 of the block: dt * 64 + lane
+  const int at4 = W == 1 ? (blockIdx.x & 7) * 256 + threadIdx.x  // float4 of the block: dt * 64 + lane
+                         : (blockIdx.x & 31) * 64 + (threadIdx.x & 63);
   const int lane = at4 & 63, c = lane & 15, q = lane >> 4, dt = at4 >> 6;
   const int row = D_ROWS * rb + c, rows = a.Sq * a.H;
-  if (row >= rows) return;
   // slot of workgroup i's segment: its second only where its range began before this block
   auto slot = [&](int i) { return (2 * (int64_t)i + (i == i0 && i0 * step < s ? 1 : 0)) * RB + w; };
   float m = -INFINITY, l = 0.f;
   v4f_t acc = {0.f, 0.f, 0.f, 0.f};
-  // four partials in flight; the running maximum rescales (a NaN partial reaches the result)
-  for (int i = i0; i <= i1; i += 4) {
+  auto add = [&](float m1, float l1, v4f_t v1) {
+    if (l1 == 0.f) return;  // the row saw no key there (a NaN sum goes on)
+    const float mn = fmaxf(m, m1), ref = mn == -INFINITY ? 0.f : mn;
+    const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(m1 - ref);
+    l = l * f0 + l1 * f1;
+    acc = acc * f0 + v1 * f1;
+    m = mn;
+  };
+  // four partials in flight; the running maximum rescales
+  const int cnt = i1 - i0 + 1;
+  const int lo = i0 + (W == 1 ? 0 : cnt * wave / W), hi = i0 + (W == 1 ? cnt : cnt * (wave + 1) / W);
+  for (int i = lo; i < hi; i += 4) {
     float ms[4], ls[4];
     v4f_t v[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int64_t at = slot(min(i + j, i1));
+      const int64_t at = slot(min(i + j, hi - 1));
       ms[j] = a.ml[(at * D_ROWS + c) * 2];
       ls[j] = a.ml[(at * D_ROWS + c) * 2 + 1];
       v[j] = reinterpret_cast<const v4f_t*>(a.part + at * D_PART)[at4];
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (i + j > i1 || ms[j] == -INFINITY) continue;
-      const float mn = fmaxf(m, ms[j]);
-      const float f0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-      const float f1 = __builtin_amdgcn_exp2f(ms[j] - mn);
-      l = l * f0 + ls[j] * f1;
-      acc = acc * f0 + v[j] * f1;
-      m = mn;
+    for (int j = 0; j < 4; ++j)
+      if (i + j < hi) add(ms[j], ls[j], v[j]);
+  }
+  if constexpr (W > 1) {
+    if (wave > 0) {
+      float* r = red[wave - 1][lane];
+      r[0] = m; r[1] = l;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[2 + j] = acc[j];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int x = 0; x < W - 1; ++x) {
+      const float* r = red[x][lane];
+      add(r[0], r[1], v4f_t{r[2], r[3], r[4], r[5]});
     }
   }
+  if (row >= rows) return;
   const float il = l == 0.f ? 0.f : 1.f / l;
   uint2 pk;
   pk.x = pack_dt<DT>(acc[0] * il, acc[1] * il);
@@ -834,13 +855,16 @@ struct DecPlan {
   int rb, nrb, ny, wgs;
 };
 // RB row blocks per workgroup (all heads of a token share its key tiles); as many workgroups as the
-// chip holds at once: one of 8 waves per CU (144 KB of stages), two of fewer
+// chip holds at once, one of 8 waves per CU (144 KB of stages), two of fewer; and no more than
+// D_CUTS per line of tiles, since each leaves a partial output (one sequence of 4000 tokens, 128
+// heads: 29 us, 35 with a workgroup for each of its 125 tiles, 32 with 24)
 DecPlan dec_plan(int64_t B, int64_t rows, int64_t maxlen) {
   DecPlan p;
   p.nrb = (int)((rows + D_ROWS - 1) / D_ROWS);
   p.rb = p.nrb <= 1 ? 1 : p.nrb <= 2 ? 2 : p.nrb <= 4 ? 4 : 8;
   p.ny = (p.nrb + p.rb - 1) / p.rb;
-  const int64_t most = (B * p.ny * ((maxlen + DKT - 1) / DKT) + D_MIN - 1) / D_MIN;
+  const int64_t lines = B * p.ny, tiles = (maxlen + DKT - 1) / DKT;
+  const int64_t most = lines * (tiles < D_CUTS ? tiles : D_CUTS);
   const int64_t fit = p.rb == 8 ? 256 : 512;
   p.wgs = (int)(most < fit ? most : fit);
   return p;
@@ -856,7 +880,14 @@ int launch_dec(const MlaDecArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((k_mla_dec<DT, RB, NST>), dim3((unsigned)a.wgs), 64 * RB, lds, st, a);
   if (int rc = check_launch("lcq_mla_decode")) return rc;
   if (a.wgs == 1) return LCQ_OK;
-  hipLaunchKernelGGL((k_mla_join<DT, RB>), dim3((unsigned)a.nrb * 8, (unsigned)a.B), 256, 0, st, a);
+  // the mean number of partials of a row block decides (one sequence of 4000 tokens, 16 heads: 17
+  // against 26 us for both kernels; 32 sequences of 8192, 3 partials each: 177 against 161)
+  if (a.wgs >= 8 * a.B * a.ny)
+    hipLaunchKernelGGL((k_mla_join<DT, RB, 4>), dim3((unsigned)a.nrb * 32, (unsigned)a.B), 256, 0, st,
+                       a);
+  else
+    hipLaunchKernelGGL((k_mla_join<DT, RB, 1>), dim3((unsigned)a.nrb * 8, (unsigned)a.B), 256, 0, st,
+                       a);
   return check_launch("lcq_mla_decode");
 }
 

@@ -231,3 +231,25 @@ def test_other_stream_and_graph(dev):
         torch.cuda.synchronize()
         assert torch.equal(a, ops.mla_decode(ql, qr, ckv, kr, table, n, SCALE))
         assert torch.equal(b, ops.mla_fwd_causal(*x, SCALE))
+
+
+@pytest.mark.parametrize('B,H,n', [(1, 16, 40), (1, 16, 700), (1, 20, 4500), (9, 128, 900)])
+def test_decode_nan_row(dev, B, H, n):
+    """A NaN query gives NaN outputs, for its row alone, however many workgroups share the keys."""
+    from lightcompress_amd import ops
+    g = torch.Generator().manual_seed(n)
+    ps = 16
+    nb = -(-n // ps)
+    ckv = torch.randn(B * nb, ps, 512, generator=g).bfloat16().to(dev)
+    kr = torch.randn(B * nb, ps, 64, generator=g).bfloat16().to(dev)
+    table = torch.arange(B * nb, dtype=torch.int32).view(B, nb).to(dev)
+    lens = torch.full((B,), n, dtype=torch.int32).to(dev)
+    ql = torch.randn(B, 1, H, 512, generator=g).bfloat16().to(dev)
+    qr = torch.randn(B, 1, H, 64, generator=g).bfloat16().to(dev)
+    want = ops.mla_decode(ql, qr, ckv, kr, table, lens, SCALE)
+    assert not want.isnan().any()
+    ql[B - 1, 0, 3, 100] = float('nan')
+    got = ops.mla_decode(ql, qr, ckv, kr, table, lens, SCALE)
+    assert got[B - 1, 0, 3].isnan().all() and got.isnan().sum() == 512
+    got[B - 1, 0, 3] = want[B - 1, 0, 3]
+    assert torch.equal(got, want)
