@@ -238,3 +238,53 @@ def test_other_stream_and_graph(dev):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, ops.int4_linear(x, *w))
+
+
+def test_streams_at_once_and_graphs_with_workspaces(dev):
+    """Products whose k is split, on two streams at once and in two graphs replayed in turn: each
+    has its own partial sums."""
+    from lightcompress_amd import ops
+    g = torch.Generator().manual_seed(31)
+    cases = []
+    for m, n, k in ((37, 200, 4096), (2, 136, 9216)):
+        w = weight(g, 'autoawq', n, k, 128, dev)
+        xs = [acts(g, m, k, dt=torch.bfloat16, dev=dev) for _ in range(3)]
+        cases.append((w, xs, [ops.int4_linear(x, *w) for x in xs]))
+        y, tol = R.linear(xs[0], *w)
+        assert R.close(cases[-1][2][0], y, tol)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for i in range(3):
+        for s, (w, xs, _) in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(ops.int4_linear(xs[i], *w))
+    torch.cuda.synchronize()
+    for j, y in enumerate(got):
+        assert torch.equal(y, cases[j % 2][2][j // 2])
+    graphs = []
+    for w, xs, _ in cases:
+        xi = xs[0].clone()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            y = ops.int4_linear(xi, *w)
+        graphs.append((gr, xi, y))
+    for i in (1, 2, 0, 1):
+        for (gr, xi, _), (w, xs, _) in zip(graphs, cases):
+            xi.copy_(xs[i])
+            gr.replay()
+            ops.int4_linear(xs[(i + 1) % 3], *w)
+        torch.cuda.synchronize()
+        for (_, _, y), (_, _, want) in zip(graphs, cases):
+            assert torch.equal(y, want[i])
+
+
+@pytest.mark.parametrize('layout', LAYOUTS)
+def test_nothing_to_do(dev, layout):
+    from lightcompress_amd import ops
+    w = weight(torch.Generator().manual_seed(1), layout, 64, 256, 64, dev)
+    x = torch.zeros(0, 256, dtype=torch.bfloat16, device=dev)
+    assert ops.int4_linear(x, *w).shape == (0, 64)
+    assert ops.int4_linear(x.view(2, 0, 256), *w).shape == (2, 0, 64)
+    tab = ops.int4_weight_table([w], dev)
+    off = torch.zeros(2, dtype=torch.int64, device=dev)
+    assert ops.int4_linear_grouped(x, off, tab, 64, 64, layout=layout).shape == (0, 64)

@@ -253,3 +253,85 @@ def test_decode_nan_row(dev, B, H, n):
     assert got[B - 1, 0, 3].isnan().all() and got.isnan().sum() == 512
     got[B - 1, 0, 3] = want[B - 1, 0, 3]
     assert torch.equal(got, want)
+
+
+def paged(g, B, lens, H, Sq, ps, dt, dev, spare=3):
+    """A cache whose pages are dealt out in a random order, tables wider than any length."""
+    nb = max(-(-max(lens) // ps), 1) + spare
+    P = B * nb + 5
+    ckv = torch.randn(P, ps, 512, generator=g).to(dt).to(dev)
+    kr = torch.randn(P, ps, 64, generator=g).to(dt).to(dev)
+    table = torch.randperm(P, generator=g)[:B * nb].to(torch.int32).view(B, nb).to(dev)
+    ql = torch.randn(B, Sq, H, 512, generator=g).to(dt).to(dev)
+    qr = torch.randn(B, Sq, H, 64, generator=g).to(dt).to(dev)
+    return ql, qr, ckv, kr, table, torch.tensor(lens, dtype=torch.int32).to(dev)
+
+
+@pytest.mark.parametrize('lens,H,Sq,spare', [
+    ([(7 * i) % 90 for i in range(70)], 16, 1, 0),            # more sequences than a wave's lanes
+    ([0] * 66 + [300, 0, 1], 5, 3, 2), ([33, 64], 128, 3, 900),   # a table far wider than lengths
+    ([1700] * 3 + [0, 2100], 16, 1, 0), ([1], 1, 1, 0)])
+def test_decode_many_sequences_wide_tables(dev, lens, H, Sq, spare):
+    from lightcompress_amd import ops
+    g = torch.Generator().manual_seed(len(lens) + H)
+    x = paged(g, len(lens), lens, H, Sq, 16, torch.bfloat16, dev, spare)
+    got = ops.mla_decode(*x, SCALE)
+    y, tol = R.decode(*x, SCALE)
+    assert R.close(got, y, tol)
+    assert torch.equal(got, ops.mla_decode(*x, SCALE))
+
+
+def test_nothing_to_do(dev):
+    from lightcompress_amd import ops
+    g = torch.Generator().manual_seed(2)
+    x = prefill_inputs(g, 2, 3, 5, 9, torch.bfloat16, dev)
+    assert ops.mla_fwd_causal(*[t[:0] for t in x], SCALE).shape == (0, 5, 3, 128)
+    assert ops.mla_fwd_causal(x[0][:, :, :0], x[1][:, :, :0], *x[2:], SCALE).shape == (2, 0, 3, 128)
+    z = paged(g, 2, [5, 9], 4, 1, 16, torch.bfloat16, dev)
+    out = ops.mla_decode(z[0][:0], z[1][:0], z[2], z[3], z[4][:0], z[5][:0], SCALE)
+    assert out.shape == (0, 1, 4, 512)
+
+
+def test_streams_at_once_and_graphs_with_workspaces(dev):
+    """Split prefill and decode on two streams at once; two graphs of them replayed in turn on new
+    inputs, with eager work between: each has its own partial outputs."""
+    from lightcompress_amd import ops
+    g = torch.Generator().manual_seed(12)
+    f = [list(prefill_inputs(g, 1, 4, 60, 1500, torch.bfloat16, dev)) for _ in range(3)]
+    d = [paged(torch.Generator().manual_seed(5), 2, [900, 1300], 16, 1, 16, torch.bfloat16, dev)
+         for _ in range(3)]
+    for i in range(3):
+        d[i][0].normal_()
+    want = [(ops.mla_fwd_causal(*f[i], SCALE), ops.mla_decode(*d[i], SCALE)) for i in range(3)]
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = []
+    for i in range(3):
+        with torch.cuda.stream(s1):
+            a = ops.mla_fwd_causal(*f[i], SCALE)
+        with torch.cuda.stream(s2):
+            b = ops.mla_decode(*d[i], SCALE)
+        outs.append((a, b))
+    torch.cuda.synchronize()
+    for (a, b), (x, y) in zip(outs, want):
+        assert torch.equal(a, x) and torch.equal(b, y)
+    fi, di = [t.clone() for t in f[0]], [t.clone() for t in d[0]]
+    graphs, res = [], []
+    for fn, arg in ((ops.mla_fwd_causal, fi), (ops.mla_decode, di)):
+        fn(*arg, SCALE)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            res.append(fn(*arg, SCALE))
+        graphs.append(gr)
+    for i in (1, 2, 0, 1):
+        for t, u in zip(fi, f[i]):
+            t.copy_(u)
+        for t, u in zip(di, d[i]):
+            t.copy_(u)
+        graphs[0].replay()
+        ops.mla_decode(*d[(i + 1) % 3], SCALE)
+        graphs[1].replay()
+        ops.mla_fwd_causal(*f[(i + 1) % 3], SCALE)
+        torch.cuda.synchronize()
+        assert torch.equal(res[0], want[i][0]) and torch.equal(res[1], want[i][1])

@@ -68,10 +68,12 @@ def strides(*v):
 
 
 def fwd(lib, dtype=N.BF16, B=1, H=2, Sq=8, Skv=8, scale=0.1, qn=P, kn_s=(4096, 256, 512),
-        q_start=None, kr_s=(512, 64), out=P):
+        q_start=None, kr_s=(512, 64), out=P, ws=P, wsb=None):
+    need = lib.lcq_mla_fwd_causal_workspace_bytes(B, H, Sq, Skv)
     q, kr = strides(4096, 192, 384), strides(*kr_s)
     rc = lib.lcq_mla_fwd_causal(qn, q, P, q, P, strides(*kn_s), P, kr, P, strides(4096, 256, 512),
-                                dtype, B, H, Sq, Skv, q_start, None, scale, out, None)
+                                dtype, B, H, Sq, Skv, q_start, None, scale, out, ws,
+                                need if wsb is None else wsb, None)
     return rc, lib.lcq_last_error().decode()
 
 
@@ -81,6 +83,8 @@ def fwd(lib, dtype=N.BF16, B=1, H=2, Sq=8, Skv=8, scale=0.1, qn=P, kn_s=(4096, 2
     (dict(scale=float('inf')), 'scale'), (dict(qn=None), 'null'), (dict(qn=P + 4), 'aligned'),
     (dict(kn_s=(4096, 256, 516)), 'multiples of 8'), (dict(kn_s=(4096, 256, -512)), '2^24'),
     (dict(kr_s=(512, 1 << 24)), '2^24'), (dict(Sq=9), 'q_start'), (dict(B=1 << 25), 'large'),
+    (dict(B=1 << 20, H=1 << 20), 'large'), (dict(Skv=4096, wsb=0), 'workspace'),
+    (dict(Skv=4096, ws=None), 'workspace'), (dict(Skv=4096, ws=P + 8), 'workspace'),
     (dict(Sq=1 << 29, Skv=1 << 29), 'too long')])
 def test_mla_fwd_refuses(lib, kw, msg):
     rc, err = fwd(lib, **kw)
