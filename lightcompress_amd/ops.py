@@ -7,6 +7,7 @@ through ``_native``. There is no CPU path: CPU tensors raise ``LcqError``.
 from __future__ import annotations
 
 
+import array
 import torch
 
 from . import _native as N
@@ -1587,10 +1588,8 @@ def _mla_checked(ref, dtype_of, **index):
 def _strides(*ts):
     """(keep, pointers): the leading strides of each tensor (all dims but the last) in one host
     int64 array."""
-    import ctypes
-    flat = [s for t in ts for s in t.stride()[:-1]]
-    keep = (ctypes.c_int64 * len(flat))(*flat)
-    at, out = ctypes.addressof(keep), []
+    keep = array.array('q', [s for t in ts for s in t.stride()[:-1]])
+    at, out = keep.buffer_info()[0], []
     for t in ts:
         out.append(at)
         at += 8 * (t.dim() - 1)
