@@ -238,7 +238,9 @@ __device__ __forceinline__ void i4_stage(const I4Args& a, const I4Cols<LA, 4>& c
 // k split over its W waves (and, one matrix only, over a.nsplit workgroups), every word used by
 // one wave. vLLM words go straight from memory to the MFMA operands; AutoAWQ words through a
 // wave's own LDS stage, whose transposed reads form the fragments. The waves' partial tiles are
-// summed through LDS in a fixed order.
+// summed through LDS in a fixed order. What bounds it: one row, the latency of a wave's few units
+// (1 x 4096 x 4096 5.5 us); many words, memory (64 experts' gate and up, 2048 x 7168: 4.2 TB/s);
+// more rows, x's fragments, which every wave loads (37 x 14336 x 4096: 21 us, 1.5 TB/s).
 template <int DT, int LAYOUT, int F, int MT, int NT, int SETS, int W>
 struct I4Few {
   static constexpr int T = NT * SETS;
@@ -483,7 +485,9 @@ __global__ __launch_bounds__(64 * W) void k_int4_few(I4Args a) {
 // scaling a tile's products while the next one's run. vLLM: 128 x 32 a wave, words straight to
 // registers, x put into the words' element order on its way to LDS. AutoAWQ: 64 x 64 a wave, words
 // through LDS too (a transposed read gives 64 columns). The sums of x of the next unit's groups are
-// formed one unit ahead, one row tile by each wave.
+// formed one unit ahead, one row tile by each wave. What bounds it: MFMA 44 % and vector
+// instructions 39 % of the issue slots (half of those unpack and scale), at the clock the card
+// keeps under them: 2048 x 14336 x 4096 in 282 us, 850 TF/s, 0.66 of a plain bf16 product's rate.
 constexpr int TM = 128, TX = TM * 256, TW = 128 * 128;  // rows; bytes of an x, a word buffer
 
 template <int LAYOUT>
@@ -816,22 +820,34 @@ __global__ __launch_bounds__(256) void k_int4_join(I4Args a) {
   }
 }
 
-// The 128-row kernel runs where its tiles are mostly full and fill the chip, except on AutoAWQ
-// weights whose rows of words are not 16-byte aligned (LDS-DMA)
+// The 128-row kernel runs where its tiles cost less than k_int4_few's passes over the words. One
+// matrix, k 4096: a round of 128 x 256 tiles over the chip takes 63 us however few rows they hold,
+// k_int4_few about 25 us per 64 rows of 14336 columns (128 rows 51 us, 256 rows 95; of 4096
+// columns 400 rows 49). Groups (2048 x 2048 each, sets 1 / 2): vLLM 48 rows each, 64 groups: 111 /
+// 233 us against 140 / 252, but 16 groups leave CUs idle: 67 / 135 against 55 / 107, from 64 rows on
+// 68 / 137 against 85 / 132; AutoAWQ, whose small kernel costs less: one set 64 rows 130 against
+// 159, 48 rows 128 against 121; two sets 100 rows 394 against 346, 128 rows 394 against 412. Not
+// for AutoAWQ weights whose rows of words are not 16-byte aligned (LDS-DMA).
+bool i4_tile_one(int64_t m, int64_t n, int layout) {
+  return !(layout == LA && n % 32) && m > 64 && (m + TM - 1) / TM * ((n + 255) / 256) >= 96;
+}
 bool i4_use_tile(const I4Args& a, int layout, int sets) {
+  if (!a.row_off) return i4_tile_one(a.m, a.n, layout);
   if (layout == LA && a.n % 32) return false;
   const int64_t cols = sets == 2 ? 128 : 256, nblk = (a.n + cols - 1) / cols;
-  if (a.row_off) return a.m >= 48 * (int64_t)a.G;
-  return a.m > 64 && (a.m + TM - 1) / TM * nblk >= 96;
+  const int64_t least = layout == LA ? (sets == 2 ? 120 : 56) : a.G * nblk >= 512 ? 40 : 64;
+  return a.m >= least * a.G;
 }
 
-// How one matrix's k is split over workgroups (a function of the shape alone): where the column
-// blocks leave CUs without a workgroup, and up to 16 rows only where the waves have units enough to
-// pay for the join. 1 x 4096 x 14336 AutoAWQ, 64 blocks: 16.5 us with 4 splits, 28.9 without, 17.6
-// with 8; at k 4096 8.9 with 2, 7.7 without. 37 x 4096 x 14336: 25 us with 4, 54 without, 31 with 8.
+// How one matrix's k is split over workgroups (a function of the shape alone): where the blocks of
+// rows and columns leave CUs without a workgroup, and up to 16 rows only where the waves have units
+// enough to pay for the join. 1 x 4096 x 14336 AutoAWQ, 64 blocks: 16.5 us with 4 splits, 28.9
+// without, 17.6 with 8; at k 4096 8.9 with 2, 7.7 without. 37 x 4096 x 14336: 25 us with 4, 54
+// without, 31 with 8. 128 x 1024 x 4096: 14.5 us with 8, 23.6 without.
 int i4_nsplit(int64_t m, int64_t n, int64_t k, int layout) {
-  if (m > 64) return 1;
-  const int64_t nt = m > 16 ? 4 : i4_few_tiles(layout, n), blocks = (n + 16 * nt - 1) / (16 * nt);
+  if (i4_tile_one(m, n, layout)) return 1;
+  const int64_t nt = m > 16 ? 4 : i4_few_tiles(layout, n);
+  const int64_t blocks = (n + 16 * nt - 1) / (16 * nt) * ((m + 63) / 64);
   const int64_t upw = ((k + 127) / 128 + 7) / 8;  // units per wave of a workgroup
   if (m <= 16 && upw <= (layout == LA ? 6 : 8)) return 1;
   const int64_t most = m > 16 ? upw : upw / 2, fit = 256 / blocks;
@@ -952,7 +968,8 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 using namespace lcq;
 
 extern "C" int64_t lcq_int4_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k, int layout) {
-  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  constexpr int64_t big = int64_t(1) << 31;
+  if (m <= 0 || n <= 0 || k <= 0 || m >= big || n >= big || k >= big) return 0;
   const int s = i4_nsplit(m, n, k, layout);
   return s > 1 ? 4 * s * m * n : 0;
 }

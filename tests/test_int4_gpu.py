@@ -240,6 +240,16 @@ def test_other_stream_and_graph(dev):
             assert torch.equal(out, ops.int4_linear(x, *w))
 
 
+@pytest.mark.parametrize('layout', LAYOUTS)
+@pytest.mark.parametrize('m,n,k,group', [
+    (65, 136, 4096, 128), (130, 1000, 3200, 64), (257, 72, 2080, 32), (600, 40, 1536, 128)])
+def test_linear_more_rows_split(dev, layout, m, n, k, group):
+    """More than 64 rows of few columns: several row tiles, k split over workgroups."""
+    from lightcompress_amd import _native as N
+    assert N.load().lcq_int4_gemm_workspace_bytes(m, n, k, LAYOUTS.index(layout)) > 0
+    check_linear(dev, layout, torch.bfloat16, m, n, k, group)
+
+
 def test_streams_at_once_and_graphs_with_workspaces(dev):
     """Products whose k is split, on two streams at once and in two graphs replayed in turn: each
     has its own partial sums."""

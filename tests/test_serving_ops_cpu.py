@@ -161,3 +161,16 @@ def test_python_checks():
                       (3, c[:2, :, 512:], ValueError), (0, ql.half(), TypeError)):
         with pytest.raises(err):
             ops.mla_decode(*good[:i], v, *good[i + 1:], 0.1)
+
+
+def test_workspace_sizes_of_any_shape(lib):
+    """Never negative, zero for shapes the products refuse."""
+    for v in (-1, 0, 1, 64, 1 << 20, (1 << 31) - 1, 1 << 31, 1 << 40, (1 << 63) - 1):
+        for w in (-1, 0, 1, 4096, 1 << 31, 1 << 62):
+            for lay in (0, 1):
+                assert lib.lcq_int4_gemm_workspace_bytes(v, w, w, lay) >= 0
+                assert lib.lcq_int4_gemm_workspace_bytes(w, v, 4096, lay) >= 0
+            assert lib.lcq_mla_fwd_causal_workspace_bytes(v, w, w, v) >= 0
+            assert lib.lcq_mla_fwd_causal_workspace_bytes(w, 1, v, w) >= 0
+            assert lib.lcq_mla_decode_workspace_bytes(v, 1, w, w) >= 0
+            assert lib.lcq_mla_decode_workspace_bytes(1, w, 1, v) >= 0
