@@ -173,7 +173,8 @@ class ExpertList(nn.ModuleList):
         from .module_utils import int4_weight
         ws = [[int4_weight(getattr(mlp, p)) for mlp in self]
               for p in ('gate_proj', 'up_proj', 'down_proj')]
-        key = tuple(None if t is None else t.data_ptr() for row in ws for w in row for t in w)
+        key = tuple(None if t is None else (t.data_ptr(), t.shape, t.dtype)
+                    for row in ws for w in row for t in w)
         cached = getattr(self, '_lcq_int4_tables', None)
         if cached is None or cached[0] != key:
             gate, up, down = (ops.int4_weight_table(row, device) for row in ws)
