@@ -298,3 +298,20 @@ def test_nothing_to_do(dev, layout):
     tab = ops.int4_weight_table([w], dev)
     off = torch.zeros(2, dtype=torch.int64, device=dev)
     assert ops.int4_linear_grouped(x, off, tab, 64, 64, layout=layout).shape == (0, 64)
+
+
+@pytest.mark.parametrize('layout', LAYOUTS)
+@pytest.mark.parametrize('m', [20, 100])
+def test_linear_split_bias_and_strided_rows(dev, layout, m):
+    """A split k with a bias (added once), rows of x inside a wider tensor, leading batch dims."""
+    from lightcompress_amd import ops
+    g = torch.Generator().manual_seed(m)
+    n, k = 72, 3200
+    w = weight(g, layout, n, k, 128, dev)
+    wide = acts(g, m, k + 64, dt=torch.float16, dev=dev)
+    x = wide[:, 32:32 + k]
+    b = (torch.randn(n, generator=g) * 3).half().to(dev)
+    y, tol = R.linear(x, *w, bias=b)
+    got = ops.int4_linear(x, *w, bias=b)
+    assert R.close(got, y, tol)
+    assert torch.equal(got, ops.int4_linear(x.reshape(2, m // 2, k), *w, bias=b).view(m, n))
