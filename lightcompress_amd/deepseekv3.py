@@ -256,10 +256,11 @@ def _plain_weight(lin):
     return wb[0]
 
 
-def _lcq_mla_ok(attn, x, attention_mask, past_key_values, kwargs) -> bool:
-    """The cases the lcq latent attention takes: causal without a mask (a prompt with no cached
-    tokens, or one new token), no dropout or attention weights asked for, the checkpoint's head
-    dims, bf16 / fp16 on the device, no autograd."""
+def _lcq_mla_past(attn, x, attention_mask, past_key_values, kwargs):
+    """The number of tokens cached before x, for the cases the lcq latent attention takes: causal
+    without a mask (a prompt with no cached tokens, or one new token), no dropout or attention
+    weights asked for, the checkpoint's head dims, bf16 / fp16 on the device, no autograd. None for
+    anything else."""
     if (not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float16) or x.dim() != 3
             or attention_mask is not None or kwargs.get('output_attentions')
             or kwargs.get('is_causal') is False
@@ -268,9 +269,10 @@ def _lcq_mla_ok(attn, x, attention_mask, past_key_values, kwargs) -> bool:
             or attn.config._attn_implementation != 'sdpa'
             or (attn.qk_nope_head_dim, attn.qk_rope_head_dim, attn.v_head_dim,
                 attn.kv_lora_rank) != (128, 64, 128, 512)):
-        return False
-    past = past_key_values.get_seq_length(attn.layer_idx) if past_key_values is not None else 0
-    return past == 0 or x.shape[1] == 1
+        return None
+    # (a number now: a preallocated cache counts in a tensor that its update changes)
+    past = 0 if past_key_values is None else int(past_key_values.get_seq_length(attn.layer_idx))
+    return past if past == 0 or x.shape[1] == 1 else None
 
 
 def _lcq_mla_forward(self, hidden_states, position_embeddings, attention_mask,
@@ -278,11 +280,12 @@ def _lcq_mla_forward(self, hidden_states, position_embeddings, attention_mask,
     """DeepseekV3Attention.forward on the lcq latent attention: prompts in the expanded form on
     kv_b_proj's own output (no concatenated keys), one new token behind cached latents in the
     absorbed form (no up-projection of the cache) where kv_b_proj is a plain weight. Anything
-    _lcq_mla_ok does not take runs the stock forward."""
+    _lcq_mla_past does not take runs the stock forward."""
     from transformers.models.deepseek_v3 import modeling_deepseek_v3 as md
 
     from . import ops
-    if not _lcq_mla_ok(self, hidden_states, attention_mask, past_key_values, kwargs):
+    past = _lcq_mla_past(self, hidden_states, attention_mask, past_key_values, kwargs)
+    if past is None:
         return type(self).forward(self, hidden_states, position_embeddings, attention_mask,
                                   past_key_values, **kwargs)
     B, S = hidden_states.shape[:2]
@@ -303,8 +306,10 @@ def _lcq_mla_forward(self, hidden_states, position_embeddings, attention_mask,
     q_rot, k_rot = rope(q_rot, k_rot, cos, sin)
     if past_key_values is not None:
         ckv, k_rot = past_key_values.update(ckv, k_rot, self.layer_idx)
+        # a preallocated cache gives its whole buffer: the tokens so far are its first ones
+        ckv, k_rot = ckv[:, :, :past + S], k_rot[:, :, :past + S]
     T = ckv.shape[2]
-    w = _plain_weight(self.kv_b_proj) if T > S else None
+    w = _plain_weight(self.kv_b_proj) if past else None
     if w is not None and w.dtype == q.dtype:
         # one new token: q_latent = q_nope W_k per head, the attended latent times W_v^T
         w = w.view(H, -1, self.kv_lora_rank)
