@@ -256,22 +256,31 @@ def _plain_weight(lin):
     return wb[0]
 
 
-def _lcq_mla_past(attn, x, attention_mask, past_key_values, kwargs):
+def _needs_grad(tensors) -> bool:
+    return torch.is_grad_enabled() and any(
+        isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+
+
+def _lcq_mla_past(attn, x, position_embeddings, attention_mask, past_key_values, kwargs):
     """The number of tokens cached before x, for the cases the lcq latent attention takes: causal
     without a mask (a prompt with no cached tokens, or one new token), no dropout or attention
-    weights asked for, the checkpoint's head dims, bf16 / fp16 on the device, no autograd. None for
-    anything else."""
+    weights asked for, the checkpoint's head dims, bf16 / fp16 on the device, no gradient asked for
+    by a parameter, an input or a cached token. None for anything else."""
     if (not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float16) or x.dim() != 3
             or attention_mask is not None or kwargs.get('output_attentions')
             or kwargs.get('is_causal') is False
             or (attn.training and attn.attention_dropout)
-            or (torch.is_grad_enabled() and any(p.requires_grad for p in attn.parameters()))
+            or _needs_grad([x, *position_embeddings, *attn.parameters()])
             or attn.config._attn_implementation != 'sdpa'
             or (attn.qk_nope_head_dim, attn.qk_rope_head_dim, attn.v_head_dim,
                 attn.kv_lora_rank) != (128, 64, 128, 512)):
         return None
     # (a number now: a preallocated cache counts in a tensor that its update changes)
     past = 0 if past_key_values is None else int(past_key_values.get_seq_length(attn.layer_idx))
+    if past and torch.is_grad_enabled():
+        layers = getattr(past_key_values, 'layers', [])
+        if attn.layer_idx < len(layers) and _needs_grad(vars(layers[attn.layer_idx]).values()):
+            return None
     return past if past == 0 or x.shape[1] == 1 else None
 
 
@@ -284,7 +293,8 @@ def _lcq_mla_forward(self, hidden_states, position_embeddings, attention_mask,
     from transformers.models.deepseek_v3 import modeling_deepseek_v3 as md
 
     from . import ops
-    past = _lcq_mla_past(self, hidden_states, attention_mask, past_key_values, kwargs)
+    past = _lcq_mla_past(self, hidden_states, position_embeddings, attention_mask,
+                         past_key_values, kwargs)
     if past is None:
         return type(self).forward(self, hidden_states, position_embeddings, attention_mask,
                                   past_key_values, **kwargs)
