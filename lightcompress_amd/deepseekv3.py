@@ -34,7 +34,9 @@ class ExpertList(nn.ModuleList):
         if (top_k_weights.dtype in (torch.float32, torch.bfloat16, torch.float16)
                 and self._grouped_fp8_ok(hidden_states)):
             return self._forward_grouped_fp8(hidden_states, top_k_index, top_k_weights)
+        # (the packed experts have no backward pass, but the combine's weights do in the loop below)
         if (top_k_weights.dtype in (torch.float32, torch.bfloat16, torch.float16)
+                and not _needs_grad([top_k_weights])
                 and self._grouped_int4_ok(hidden_states)):
             return self._forward_grouped_int4(hidden_states, top_k_index, top_k_weights)
         out = torch.zeros_like(hidden_states)
@@ -182,6 +184,7 @@ class ExpertList(nn.ModuleList):
             self._lcq_int4_tables = cached
         return cached[1]
 
+    @torch.no_grad()          # as the packed modules' own forward
     def _forward_grouped_int4(self, hidden_states, top_k_index, top_k_weights):
         from . import ops
         from .module_utils import int4_weight
@@ -196,11 +199,10 @@ class ExpertList(nn.ModuleList):
             _, s, z = int4_weight(lin)
             return (lin.in_features // s.shape[1 if z is None else 0],
                     'vllm' if z is None else 'autoawq')
-        with torch.no_grad():
-            flat, order = torch.sort(top_k_index.reshape(-1).to(torch.int64), stable=True)
-            row_off = torch.searchsorted(flat, torch.arange(E + 1, device=flat.device))
-            slot_row = torch.empty_like(order)                # (token, slot) -> sorted row
-            slot_row[order] = torch.arange(order.numel(), device=order.device)
+        flat, order = torch.sort(top_k_index.reshape(-1).to(torch.int64), stable=True)
+        row_off = torch.searchsorted(flat, torch.arange(E + 1, device=flat.device))
+        slot_row = torch.empty_like(order)                # (token, slot) -> sorted row
+        slot_row[order] = torch.arange(order.numel(), device=order.device)
         g, layout = kind(self[0].gate_proj)
         h = ops.int4_linear_grouped(hidden_states, row_off, gate_up, inter, g, layout,
                                     a_rows=order // k, silu_mul=True)

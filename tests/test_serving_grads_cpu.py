@@ -60,3 +60,24 @@ def test_attention_keeps_the_gradient_of_cached_tokens():
     cache = DynamicCache()
     cache.update(k.detach(), torch.zeros(1, 1, 3, 64), 0)
     assert past(attn, hidden(S=1), rotary(), cache) == 3
+
+
+def test_experts_keep_the_gradient_of_the_combine(monkeypatch):
+    """Routing weights that require a gradient: the experts run one by one, where the combine has
+    a backward pass."""
+    experts = D.ExpertList([nn.Linear(4, 4).requires_grad_(False) for _ in range(2)])
+    monkeypatch.setattr(D.ExpertList, '_grouped_fp8_ok', lambda *a: False)
+    monkeypatch.setattr(D.ExpertList, '_grouped_int4_ok', lambda *a: True)
+    monkeypatch.setattr(D.ExpertList, '_forward_grouped_int4', lambda *a: 'grouped')
+    x, idx = torch.randn(3, 4), torch.tensor([[0, 1], [1, 0], [0, 1]])
+    w = torch.rand(3, 2)
+    assert experts(x, idx, w) == 'grouped'
+    w.requires_grad_(True)
+    experts(x, idx, w).square().sum().backward()
+    out = torch.stack([experts[e](x) for e in range(2)])             # [2, 3, 4]
+    h = torch.stack([out[idx[:, j], torch.arange(3)] for j in range(2)], 1)   # [3, 2, 4]
+    y = (h * w.detach()[..., None]).sum(1)
+    # sums of 4 fp32 products of size about 1, each step off by 2^-24 of it
+    assert torch.allclose(w.grad, (2 * y[:, None] * h).sum(-1), atol=1e-5)
+    with torch.no_grad():
+        assert experts(x, idx, w) == 'grouped'
