@@ -1421,6 +1421,13 @@ def _same_device(ref: torch.Tensor, **tensors):
             raise ValueError(f'{name} is on {t.device}, not on {dev}')
 
 
+def _no_backward(name: str, *tensors):
+    """These operators have no backward pass: an input whose gradient would be lost is refused."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f'{name} has no backward pass, and an input requires a gradient: call it '
+                           'under torch.no_grad() or on detached tensors')
+
+
 def _int4_weight(qweight, scales, qzeros):
     """(layout, n, k, group) of a packed weight after checking its tensors."""
     if qweight.dtype is not torch.int32 or qweight.dim() != 2 or not qweight.is_contiguous():
@@ -1473,7 +1480,8 @@ def int4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
     codes, scales fp16 [n, k/group]). With qzeros: the AutoAWQ layout of ``pack_autoawq_gemm``
     (qweight [k, n/8], scales [k/group, n], qzeros [k/group, n/8]). The group size follows from
     the shapes (a multiple of 32). Codes enter exactly, sums are fp32, the result is rounded once
-    to x's dtype. Not differentiable."""
+    to x's dtype. Not differentiable: an input that requires a gradient is refused."""
+    _no_backward('int4_linear', x, scales, bias)
     layout, n, k, group = _int4_weight(qweight, scales, qzeros)
     x2 = _int4_x(x, k)
     if bias is not None and (bias.dtype != x.dtype or bias.dim() != 1 or bias.numel() != n
@@ -1525,7 +1533,9 @@ def int4_linear_grouped(x: torch.Tensor, row_off: torch.Tensor, wtab: torch.Tens
     x itself is sorted. wtab from int4_weight_table, [G, 3] or [2, G, 3] (two sets: gate and up of
     the same rows), all [n, k] with this group size and layout. Returns y [rows, n], or
     [2, rows, n] for two sets; ``silu_mul`` (two sets = gate, up): h [rows, n] = silu(gate) * up,
-    formed in fp32 and rounded once. Rows outside every group are not written."""
+    formed in fp32 and rounded once. Rows outside every group are not written. Not differentiable:
+    an input that requires a gradient is refused."""
+    _no_backward('int4_linear_grouped', x)
     if layout not in INT4_LAYOUTS:
         raise ValueError(f'layout must be one of {sorted(INT4_LAYOUTS)}')
     if x.dim() != 2:
@@ -1605,7 +1615,9 @@ def mla_fwd_causal(q_nope: torch.Tensor, q_rope: torch.Tensor, k_nope: torch.Ten
     projections seen head by head), k_rope [B, Skv, 64] or [B, 1, Skv, 64], one rotary key for all
     heads. Query i stands at position q_start[b] + i (int32 [B]; default Skv - Sq, the queries are
     the last tokens) and sees the keys up to its position below kv_lens[b] (int32 [B]; default
-    Skv); a query that sees none gives zeros. Returns [B, Sq, H, 128] contiguous."""
+    Skv); a query that sees none gives zeros. Returns [B, Sq, H, 128] contiguous. Not
+    differentiable: an input that requires a gradient is refused."""
+    _no_backward('mla_fwd_causal', q_nope, q_rope, k_nope, k_rope, v)
     B, H, Sq, _ = q_nope.shape
     Skv = k_nope.shape[2]
     if k_rope.dim() == 4 and k_rope.shape[1] == 1:
@@ -1643,7 +1655,9 @@ def mla_decode(q_latent: torch.Tensor, q_rope: torch.Tensor, ckv: torch.Tensor,
     one cache, or two caches; any strides with a contiguous last dim); block_table int32 [B, nb]
     names the pages of each sequence, kv_lens int32 [B] its tokens, the Sq new ones included: new
     token i sees the first kv_lens - Sq + i + 1. A page number outside the cache hides its tokens;
-    a row that sees none gives zeros. Returns the attended latents [B, Sq, H, 512] contiguous."""
+    a row that sees none gives zeros. Returns the attended latents [B, Sq, H, 512] contiguous. Not
+    differentiable: an input that requires a gradient is refused."""
+    _no_backward('mla_decode', q_latent, q_rope, ckv, k_rope)
     B, Sq, H, _ = q_latent.shape
     P, ps = ckv.shape[:2]
     _mla_checked(q_latent, dict(q_rope=q_rope, ckv=ckv, k_rope=k_rope), block_table=block_table,

@@ -2,10 +2,13 @@
 is refused or takes another path. Decided on the host, so without a GPU."""
 import types
 
+import pytest
 import torch
 import torch.nn as nn
 
+from lightcompress_amd import _native as N
 from lightcompress_amd import deepseekv3 as D
+from lightcompress_amd import ops
 
 
 def attention():
@@ -60,6 +63,33 @@ def test_attention_keeps_the_gradient_of_cached_tokens():
     cache = DynamicCache()
     cache.update(k.detach(), torch.zeros(1, 1, 3, 64), 0)
     assert past(attn, hidden(S=1), rotary(), cache) == 3
+
+
+def test_operators_refuse_inputs_that_require_a_gradient():
+    qw, s = torch.zeros(64, 32, dtype=torch.int32), torch.ones(64, 2, dtype=torch.float16)
+    x = torch.zeros(3, 256, dtype=torch.bfloat16)
+    off, rows = torch.tensor([0, 3]), torch.arange(3)
+    tab = ops.int4_weight_table([(qw, s)], 'cpu')
+    q = torch.zeros(1, 2, 4, 128, dtype=torch.bfloat16)
+    kr = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
+    ql = torch.zeros(1, 1, 2, 512, dtype=torch.bfloat16)
+    c = torch.zeros(3, 16, 576, dtype=torch.bfloat16)
+    t, n = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    bias = torch.zeros(64, dtype=torch.bfloat16)
+    calls = [
+        (lambda x, s, bias: ops.int4_linear(x, qw, s, bias=bias), (x, s, bias)),
+        (lambda x: ops.int4_linear_grouped(x, off, tab, 64, 128, a_rows=rows), (x,)),
+        (lambda *a: ops.mla_fwd_causal(*a, 0.1),
+         (q, q[..., :64].clone(), q.clone(), kr, q.clone())),
+        (lambda *a: ops.mla_decode(*a, t, n, 0.1),
+         (ql, ql[..., :64].clone(), c[..., :512].clone(), c[..., 512:].clone()))]
+    for fn, args in calls:
+        for i in range(len(args)):
+            a = [u.detach().clone().requires_grad_(j == i) for j, u in enumerate(args)]
+            with pytest.raises(RuntimeError, match='gradient'):
+                fn(*a)
+            with torch.no_grad(), pytest.raises(N.LcqError, match='GPU only'):
+                fn(*a)          # past that check
 
 
 def test_experts_keep_the_gradient_of_the_combine(monkeypatch):
