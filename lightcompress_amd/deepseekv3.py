@@ -68,8 +68,7 @@ class ExpertList(nn.ModuleList):
         """x fits the grouped kernels and every expert is the stock MLP with no hooks."""
         if (not len(self) or x.dim() != 2 or not x.is_cuda
                 or x.dtype != torch.bfloat16 or len(self) > 1 << 20
-                or torch.nn.modules.module._global_forward_hooks
-                or torch.nn.modules.module._global_forward_pre_hooks):
+                or _global_hooks()):
             return False
         mlp_forward = _mlp_forward()
         for mlp in self:
@@ -249,11 +248,17 @@ def unfuse_experts(model: nn.Module) -> nn.Module:
     return model
 
 
+def _global_hooks() -> bool:
+    m = torch.nn.modules.module
+    return bool(m._global_forward_hooks or m._global_forward_pre_hooks)
+
+
 def _plain_weight(lin):
     """The weight of a linear that is exactly x W^T with no hooks, None for anything else."""
     from .llama import _linear_wb
     wb = _linear_wb(lin)
-    if wb is None or wb[1] is not None or lin._forward_hooks or lin._forward_pre_hooks:
+    if (wb is None or wb[1] is not None or lin._forward_hooks or lin._forward_pre_hooks
+            or _global_hooks()):
         return None
     return wb[0]
 
