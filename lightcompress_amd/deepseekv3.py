@@ -169,7 +169,8 @@ class ExpertList(nn.ModuleList):
 
     def _int4_tables(self, device):
         """([2, E, 3] gate + up, [E, 3] down) device tables of the experts' packed buffers,
-        rebuilt when any of them changed (the modules keep the tensors)."""
+        rebuilt when any of them changed (the modules keep the tensors). A table that is replaced
+        is not reused for other memory before the streams that read it are done with it."""
         from . import ops
         from .module_utils import int4_weight
         ws = [[int4_weight(getattr(mlp, p)) for mlp in self]
@@ -178,10 +179,15 @@ class ExpertList(nn.ModuleList):
                     for row in ws for w in row for t in w)
         cached = getattr(self, '_lcq_int4_tables', None)
         if cached is None or cached[0] != key:
-            gate, up, down = (ops.int4_weight_table(row, device) for row in ws)
-            cached = (key, (torch.stack([gate, up]).contiguous(), down))
+            gate, up, down = ws
+            cached = (key, (ops.int4_weight_table(gate, device, up),
+                            ops.int4_weight_table(down, device)))
             self._lcq_int4_tables = cached
-        return cached[1]
+        tables = cached[1]
+        if device.type == 'cuda':
+            for t in tables:
+                t.record_stream(torch.cuda.current_stream(device))
+        return tables
 
     @torch.no_grad()          # as the packed modules' own forward
     def _forward_grouped_int4(self, hidden_states, top_k_index, top_k_weights):

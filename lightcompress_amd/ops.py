@@ -1501,26 +1501,32 @@ def int4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
     return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
 
 
-def int4_weight_table(weights, device) -> torch.Tensor:
+def int4_weight_table(weights, device, up=None) -> torch.Tensor:
     """Device table [G, 3] int64 of (qweight, scales, qzeros) addresses for int4_linear_grouped,
     after checking every entry: tuples (qweight, scales) or (qweight, scales, None) in the vLLM
-    layout, (qweight, scales, qzeros) in the AutoAWQ one, all of one layout, shape and group. The
+    layout, (qweight, scales, qzeros) in the AutoAWQ one, all of one layout, shape and group. With
+    a second set ``up`` of as many weights: [2, G, 3]. The table is made on the host and whole on
+    the device when this returns (any stream may read it; not while a graph is captured). The
     tensors must outlive every launch that reads the table (the caller keeps them with it)."""
-    rows, shape = [], None
+    sets, shape = [weights] if up is None else [weights, up], None
+    rows = []
     device = torch.device(device)
-    for w in weights:
-        qw, s, z = w if len(w) == 3 else (*w, None)
-        got = _int4_weight(qw, s, z)
-        if shape is None:
-            shape = got
-        if got != shape:
-            raise ValueError(f'grouped int4 weights differ: {got} vs {shape}')
-        if qw.device.type != device.type or (device.index is not None and qw.device != device):
-            raise ValueError(f'grouped int4 weights on {qw.device}, table on {device}')
-        rows.append((qw.data_ptr(), s.data_ptr(), z.data_ptr() if z is not None else 0))
-    if not rows:
-        raise ValueError('no weights')
-    return torch.tensor(rows, dtype=torch.int64).to(device)
+    for ws in sets:
+        rows.append([])
+        for w in ws:
+            qw, s, z = w if len(w) == 3 else (*w, None)
+            got = _int4_weight(qw, s, z)
+            if shape is None:
+                shape = got
+            if got != shape:
+                raise ValueError(f'grouped int4 weights differ: {got} vs {shape}')
+            if (qw.device.type != device.type
+                    or (device.index is not None and qw.device != device)):
+                raise ValueError(f'grouped int4 weights on {qw.device}, table on {device}')
+            rows[-1].append((qw.data_ptr(), s.data_ptr(), z.data_ptr() if z is not None else 0))
+    if not rows[0] or len(rows[0]) != len(rows[-1]):
+        raise ValueError(f'{[len(r) for r in rows]} weights: none, or not as many in both sets')
+    return torch.tensor(rows if up is not None else rows[0], dtype=torch.int64).to(device)
 
 
 def int4_linear_grouped(x: torch.Tensor, row_off: torch.Tensor, wtab: torch.Tensor, n: int,
