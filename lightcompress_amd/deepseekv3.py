@@ -170,7 +170,8 @@ class ExpertList(nn.ModuleList):
     def _int4_tables(self, device):
         """([2, E, 3] gate + up, [E, 3] down) device tables of the experts' packed buffers,
         rebuilt when any of them changed (the modules keep the tensors). A table that is replaced
-        is not reused for other memory before the streams that read it are done with it."""
+        is not reused for other memory before the streams that read it are done with it, and never
+        one that a graph was captured with."""
         from . import ops
         from .module_utils import int4_weight
         ws = [[int4_weight(getattr(mlp, p)) for mlp in self]
@@ -187,6 +188,10 @@ class ExpertList(nn.ModuleList):
         if device.type == 'cuda':
             for t in tables:
                 t.record_stream(torch.cuda.current_stream(device))
+            if torch.cuda.is_current_stream_capturing():
+                kept = self.__dict__.setdefault('_lcq_int4_captured', [])
+                if not any(t is tables for t in kept):
+                    kept.append(tables)
         return tables
 
     @torch.no_grad()          # as the packed modules' own forward

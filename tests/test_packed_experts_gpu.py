@@ -72,3 +72,31 @@ def test_experts_on_streams_of_their_own(dev, fmt, weight):
         setattr(lin, name, old)
         assert torch.equal(experts(x, idx, w), want)
         assert len(fill) == 399
+
+
+@pytest.mark.parametrize('fmt,weight', FORMATS)
+def test_experts_graph_outlives_a_replaced_buffer(dev, fmt, weight):
+    """A graph captured with the old buffers (which the caller keeps) still runs on them."""
+    E, H, inter, k, T = 8, 512, 384, 3, 2
+    experts = experts_of(dev, fmt, weight, E, H, inter, seed=4)
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(T, H, generator=g).to(torch.bfloat16).to(dev)
+    idx = torch.stack([torch.randperm(E, generator=g)[:k] for _ in range(T)]).to(dev)
+    w = torch.rand(T, k, generator=g).to(dev)
+    name = 'qweight' if fmt == 'autoawq_quant' else 'weight_packed'
+    with torch.no_grad():
+        want = experts(x, idx, w)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = experts(x, idx, w)
+        old = [getattr(e.up_proj, name) for e in experts]
+        for e, t in zip(experts, old):
+            setattr(e.up_proj, name, torch.zeros_like(t))
+        zero = experts(x, idx, w)
+        fill = [torch.zeros(n, dtype=torch.int64, device=dev) for n in range(1, 400)]
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            assert torch.equal(experts(x, idx, w), zero) and not torch.equal(zero, want)
+        assert len(fill) == 399
