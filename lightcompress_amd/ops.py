@@ -1501,7 +1501,44 @@ def int4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
     return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
 
 
-def int4_weight_table(weights, device, up=None) -> torch.Tensor:
+class Int4Table(torch.Tensor):
+    """Addresses of packed weights, and in ``int4`` what they lead to: (layout, n, k, group). What
+    torch makes of tables (stack, slices, copies) is a table of the same weights, of none where
+    they differ (``int4`` None)."""
+
+    int4 = None
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        out = super().__torch_function__(func, types, args, kwargs or {})
+        if isinstance(out, Int4Table):
+            flat = [u for t in args for u in (t if isinstance(t, (list, tuple)) else (t,))]
+            kinds = {t.int4 for t in flat if isinstance(t, Int4Table)}
+            out.int4 = kinds.pop() if len(kinds) == 1 else None
+        return out
+
+    def __deepcopy__(self, memo):
+        memo[id(self)] = out = self.clone()
+        return out
+
+
+def _int4_table(wtab, kind):
+    """(sets, groups, address) of a table after checking that its weights are `kind`."""
+    with torch._C.DisableTorchFunctionSubclass():
+        if (wtab.dtype != torch.int64 or wtab.dim() not in (2, 3) or wtab.shape[-1] != 3
+                or wtab.dim() == 3 and wtab.shape[0] not in (1, 2) or not wtab.is_contiguous()):
+            raise ValueError('wtab must be contiguous int64 [G, 3] or [2, G, 3]')
+        has = getattr(wtab, 'int4', None)
+        if has is None:
+            raise ValueError('wtab must come from int4_weight_table, or be put together from such '
+                             'tables of weights alike: bare addresses do not say what they lead to')
+        if has != kind:
+            raise ValueError('wtab holds {} weights [{}, {}] of group {}, not {} [{}, {}] of group '
+                             '{}'.format(*has, *kind))
+        return 1 if wtab.dim() == 2 else wtab.shape[0], wtab.shape[-2], wtab.data_ptr()
+
+
+def int4_weight_table(weights, device, up=None) -> Int4Table:
     """Device table [G, 3] int64 of (qweight, scales, qzeros) addresses for int4_linear_grouped,
     after checking every entry: tuples (qweight, scales) or (qweight, scales, None) in the vLLM
     layout, (qweight, scales, qzeros) in the AutoAWQ one, all of one layout, shape and group. With
@@ -1526,7 +1563,10 @@ def int4_weight_table(weights, device, up=None) -> torch.Tensor:
             rows[-1].append((qw.data_ptr(), s.data_ptr(), z.data_ptr() if z is not None else 0))
     if not rows[0] or len(rows[0]) != len(rows[-1]):
         raise ValueError(f'{[len(r) for r in rows]} weights: none, or not as many in both sets')
-    return torch.tensor(rows if up is not None else rows[0], dtype=torch.int64).to(device)
+    table = torch.tensor(rows if up is not None else rows[0], dtype=torch.int64).to(device)
+    table = table.as_subclass(Int4Table)
+    table.int4 = shape
+    return table
 
 
 def int4_linear_grouped(x: torch.Tensor, row_off: torch.Tensor, wtab: torch.Tensor, n: int,
@@ -1537,7 +1577,8 @@ def int4_linear_grouped(x: torch.Tensor, row_off: torch.Tensor, wtab: torch.Tens
     [G + 1] on the device (group g = rows [row_off[g], row_off[g + 1])). With ``a_rows`` (int64
     [rows] on the device) sorted row i is x[a_rows[i]] -- the gather happens in the kernel -- else
     x itself is sorted. wtab from int4_weight_table, [G, 3] or [2, G, 3] (two sets: gate and up of
-    the same rows), all [n, k] with this group size and layout. Returns y [rows, n], or
+    the same rows); it knows its weights, and any that are not [n, k] with this group size and
+    layout are refused. Returns y [rows, n], or
     [2, rows, n] for two sets; ``silu_mul`` (two sets = gate, up): h [rows, n] = silu(gate) * up,
     formed in fp32 and rounded once. Rows outside every group are not written. Not differentiable:
     an input that requires a gradient is refused."""
@@ -1548,11 +1589,7 @@ def int4_linear_grouped(x: torch.Tensor, row_off: torch.Tensor, wtab: torch.Tens
         raise ValueError('x must be 2-D')
     k = x.shape[1]
     x2 = _int4_x(x, k)
-    nsets = 1 if wtab.dim() == 2 else wtab.shape[0]
-    if (wtab.dtype != torch.int64 or wtab.dim() not in (2, 3) or wtab.shape[-1] != 3
-            or nsets not in (1, 2) or not wtab.is_contiguous()):
-        raise ValueError('wtab must be contiguous int64 [G, 3] or [2, G, 3]')
-    G = wtab.shape[-2]
+    nsets, G, at = _int4_table(wtab, (layout, n, k, group))
     if row_off.dtype != torch.int64 or row_off.numel() != G + 1 or not row_off.is_contiguous():
         raise ValueError('row_off must be contiguous int64 [G + 1]')
     if a_rows is not None and (a_rows.dtype != torch.int64 or a_rows.dim() != 1
@@ -1566,7 +1603,7 @@ def int4_linear_grouped(x: torch.Tensor, row_off: torch.Tensor, wtab: torch.Tens
     with N.on_device(x2):
         N.call('lcq_int4_gemm_grouped', x2.data_ptr(), N.dt(x2), x2.stride(0), x2.shape[0],
                None if a_rows is None else a_rows.data_ptr(), rows, row_off.data_ptr(),
-               wtab.data_ptr(), G, nsets, int(bool(silu_mul)), INT4_LAYOUTS[layout], int(group),
+               at, G, nsets, int(bool(silu_mul)), INT4_LAYOUTS[layout], int(group),
                int(n), k, y.data_ptr(), N.stream_of(x2))
     N.note_work('lcq_int4_gemm_grouped', 2.0 * rows * n * k * nsets)
     return y
