@@ -1557,8 +1557,9 @@ def int4_weight_table(weights, device, up=None) -> Int4Table:
                 shape = got
             if got != shape:
                 raise ValueError(f'grouped int4 weights differ: {got} vs {shape}')
-            if (qw.device.type != device.type
-                    or (device.index is not None and qw.device != device)):
+            if device.index is None and device.type == qw.device.type:
+                device = qw.device                 # 'cuda': where the first weight is
+            if qw.device != device:
                 raise ValueError(f'grouped int4 weights on {qw.device}, table on {device}')
             rows[-1].append((qw.data_ptr(), s.data_ptr(), z.data_ptr() if z is not None else 0))
     if not rows[0] or len(rows[0]) != len(rows[-1]):

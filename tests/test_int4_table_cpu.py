@@ -66,3 +66,22 @@ def test_a_table_stays_one_where_tensors_do():
     off = torch.zeros(G, dtype=torch.int64)                    # as many groups as row_off names
     with pytest.raises(ValueError, match='row_off'):
         ops.int4_linear_grouped(torch.zeros(5, K, dtype=torch.bfloat16), off, tab, NC, 128)
+
+
+class Elsewhere(torch.Tensor):
+    """A CPU tensor that says it is on another device."""
+    device = None
+
+
+def test_weights_of_two_devices_are_refused():
+    """'cuda' names no device: the table goes where its weights are, which is one device."""
+    def at(w, device):
+        w = [tuple(t.as_subclass(Elsewhere) for t in one) for one in w]
+        for one in w:
+            for t in one:
+                t.device = torch.device(device)
+        return w
+    a, b = at(weights('vllm'), 'cuda:0'), at(weights('vllm'), 'cuda:1')
+    for args in ((a[:1] + b[1:], 'cuda'), (a, 'cuda', b), (a, 'cuda:1')):
+        with pytest.raises(ValueError, match='cuda:'):
+            ops.int4_weight_table(*args)
