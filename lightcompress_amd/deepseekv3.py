@@ -150,7 +150,7 @@ class ExpertList(nn.ModuleList):
     # Same shape as the fp8 path on lcq_int4_gemm_grouped: one launch for gate and up of every
     # expert with the SiLU product in its epilogue (in fp32: one rounding where the per-expert
     # modules round gate, up, silu and the product), one for down, lcq_moe_combine. Nothing is read
-    # on the host, so a decode step can be captured.
+    # on the host, so a step of up to 65536 slots can be captured once the tables are there.
     def _grouped_int4_ok(self, x) -> bool:
         from .module_utils import int4_weight
         if not self._plain_mlps(x) or getattr(self[0].config, 'hidden_act', None) != 'silu':
@@ -180,6 +180,9 @@ class ExpertList(nn.ModuleList):
                     for row in ws for w in row for t in w)
         cached = getattr(self, '_lcq_int4_tables', None)
         if cached is None or cached[0] != key:
+            if _capturing():
+                raise RuntimeError('packed experts: the first call on these weights uploads their '
+                                   'addresses and cannot be captured; run the step once before')
             gate, up, down = ws
             cached = (key, (ops.int4_weight_table(gate, device, up),
                             ops.int4_weight_table(down, device)))
@@ -188,7 +191,7 @@ class ExpertList(nn.ModuleList):
         if device.type == 'cuda':
             for t in tables:
                 t.record_stream(torch.cuda.current_stream(device))
-            if torch.cuda.is_current_stream_capturing():
+            if _capturing():
                 kept = self.__dict__.setdefault('_lcq_int4_captured', [])
                 if not any(t is tables for t in kept):
                     kept.append(tables)
@@ -202,6 +205,10 @@ class ExpertList(nn.ModuleList):
         E, H = len(self), hidden_states.shape[1]
         if T == 0:
             return torch.zeros_like(hidden_states)
+        # (up to 65536 slots torch's sort is kernels and device copies alone, as its trace shows)
+        if T * k > 1 << 16 and _capturing():
+            raise RuntimeError(f'packed experts: {T * k} (token, expert) slots are too many for a '
+                               'captured graph (65536)')
         gate_up, down = self._int4_tables(hidden_states.device)
         inter = self[0].gate_proj.out_features
 
@@ -257,6 +264,10 @@ def unfuse_experts(model: nn.Module) -> nn.Module:
             experts.append(mlp)
         mod.experts = experts
     return model
+
+
+def _capturing() -> bool:
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
 
 
 def _global_hooks() -> bool:

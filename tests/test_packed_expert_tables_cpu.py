@@ -4,6 +4,7 @@ import pytest
 import torch
 import torch.nn as nn
 
+from lightcompress_amd import deepseekv3 as D
 from lightcompress_amd.deepseekv3 import ExpertList
 from lightcompress_amd.module_utils import VllmRealQuantLinear
 
@@ -72,3 +73,21 @@ def test_weight_table_of_two_sets():
     with pytest.raises(ValueError):
         ops.int4_weight_table(gate, 'cpu', [(m.weight_packed, m.weight_scale)
                                             for m in (x.down_proj for x in e)])
+
+
+def test_what_a_graph_cannot_hold_is_refused(monkeypatch):
+    """The tables are uploaded by a copy from pageable memory, and the sort of very many routes
+    clears memory by a library call: neither belongs into a captured graph."""
+    dev = torch.device('cpu')
+    monkeypatch.setattr(D, '_capturing', lambda: True)
+    experts = experts_of(2)
+    with pytest.raises(RuntimeError, match='captur'):
+        experts._int4_tables(dev)
+    monkeypatch.undo()
+    tables = experts._int4_tables(dev)
+    monkeypatch.setattr(D, '_capturing', lambda: True)
+    assert experts._int4_tables(dev) is tables
+    idx = torch.zeros(40000, 2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match='captur'):
+        experts._forward_grouped_int4(torch.zeros(40000, 256, dtype=torch.bfloat16), idx,
+                                      torch.ones(idx.shape))
