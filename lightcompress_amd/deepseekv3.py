@@ -81,7 +81,9 @@ class ExpertList(nn.ModuleList):
 
     def _grouped_fp8_ok(self, x) -> bool:
         from .module_utils import USE_FP8GEMM_TRITON_KERNEL, LlmcFp8Linear
-        if not USE_FP8GEMM_TRITON_KERNEL or not self._plain_mlps(x):
+        if (not USE_FP8GEMM_TRITON_KERNEL or not len(self)
+                or type(getattr(self[0], 'gate_proj', None)) is not LlmcFp8Linear
+                or not self._plain_mlps(x)):
             return False
         for mlp in self:
             for lin in (mlp.gate_proj, mlp.up_proj, mlp.down_proj):
@@ -153,7 +155,9 @@ class ExpertList(nn.ModuleList):
     # on the host, so a step of up to 65536 slots can be captured once the tables are there.
     def _grouped_int4_ok(self, x) -> bool:
         from .module_utils import int4_weight
-        if not self._plain_mlps(x) or getattr(self[0].config, 'hidden_act', None) != 'silu':
+        if (not len(self) or int4_weight(getattr(self[0], 'gate_proj', None)) is None
+                or not self._plain_mlps(x)
+                or getattr(self[0].config, 'hidden_act', None) != 'silu'):
             return False
         for p in ('gate_proj', 'up_proj', 'down_proj'):
             kinds = set()

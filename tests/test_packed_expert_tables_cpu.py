@@ -91,3 +91,19 @@ def test_what_a_graph_cannot_hold_is_refused(monkeypatch):
     with pytest.raises(RuntimeError, match='captur'):
         experts._forward_grouped_int4(torch.zeros(40000, 256, dtype=torch.bfloat16), idx,
                                       torch.ones(idx.shape))
+
+
+@pytest.mark.parametrize('kind,walks', [('float', 0), ('packed', 1)])
+def test_experts_are_walked_once_at_most(monkeypatch, kind, walks):
+    """Whether a call can run grouped is asked on every call: the look over all experts is made for
+    the kind the first one is, and not for experts that no grouped product takes."""
+    experts = experts_of(3)
+    if kind == 'float':
+        for e in experts:
+            e.gate_proj = e.up_proj = nn.Linear(256, 128, bias=False)
+            e.down_proj = nn.Linear(128, 256, bias=False)
+    seen = []
+    monkeypatch.setattr(ExpertList, '_plain_mlps', lambda self, x: seen.append(1))
+    x = torch.zeros(3, 256, dtype=torch.bfloat16)
+    assert not experts._grouped_fp8_ok(x) and not experts._grouped_int4_ok(x)
+    assert len(seen) == walks
