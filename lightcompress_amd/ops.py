@@ -1423,9 +1423,10 @@ def _same_device(ref: torch.Tensor, **tensors):
 
 def _no_backward(name: str, *tensors):
     """These operators have no backward pass: an input whose gradient would be lost is refused."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f'{name} has no backward pass, and an input requires a gradient: call it '
-                           'under torch.no_grad() or on detached tensors')
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f'{name} has no backward pass, and an input requires a gradient: '
+                               'call it under torch.no_grad() or on detached tensors')
 
 
 def _int4_weight(qweight, scales, qzeros):
