@@ -388,7 +388,7 @@ template <int DT, int G, int R>
 __device__ __forceinline__ void dot_rows(const float* __restrict__ xr,
                                          const float (&q)[R][G / 2], int h, float (&out)[R]) {
   // pairs written as 2-vectors; the build has no packed fp32 instructions, so each is two
-  // scalar ones (as packed ones this loop took 24.9 instead of 30.7 ms at 14336 x 4096)
+  // scalar ones (as packed ones this loop took 27.1 instead of 32.5 ms at 14336 x 4096)
   v2f a0[R], a1[R];
 #pragma unroll
   for (int j = 0; j < R; ++j) a0[j] = a1[j] = v2f{0.f, 0.f};
@@ -1495,11 +1495,11 @@ static constexpr int64_t CL_PAIR_MIN_ROWGROUPS = 65536;   // automatic choice, s
 // A/B probe hook (scripts/clip_rate.py): 0 = automatic, 1 = token-lane (scalar candidates),
 // 2 = row-lane, 3 = token-lane with LDS candidates (k_auto_clip_tw). Process-wide; not for
 // production use. Automatic: k_auto_clip_tw whenever the sampled tokens fit its 512 lanes (it
-// wins at every Llama-3-8B shape: v / o / gate,up / down 1.80 / 6.63 / 24.9 / 24.1 ms against
-// 2.44 / 10.4 / 34.5 / 35.5 for the scalar-candidate token-lane kernel and 3.25 / 8.22 / 27.1 /
-// 27.1 for k_auto_clip, profiles/r6_clip_rate_tw.txt); above 512 tokens the round-6 rule: the
-// scalar-candidate kernel below 65536 row-groups, k_auto_clip (lcq_auto_clip_search_act) from
-// there. All four give the same bits.
+// wins at every Llama-3-8B shape: v / o / gate,up / down 2.13 / 8.16 / 30.6 / 29.6 ms against
+// 2.46 / 10.5 / 34.9 / 35.7 for the scalar-candidate token-lane kernel and 3.94 / 9.98 / 32.4 /
+// 32.4 for k_auto_clip, profiles/clip_rate.txt); above 512 tokens the scalar-candidate kernel
+// below 65536 row-groups, k_auto_clip (lcq_auto_clip_search_act) from there. All four give the
+// same bits.
 static int g_clip_variant = 0;
 extern "C" int lcq_auto_clip_force_variant(int v) {
   LCQ_REQUIRE(v >= 0 && v <= 3, "variant: 0, 1, 2 or 3");

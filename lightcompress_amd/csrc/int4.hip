@@ -240,7 +240,10 @@ __device__ __forceinline__ void i4_stage(const I4Args& a, const I4Cols<LA, 4>& c
 // wave's own LDS stage, whose transposed reads form the fragments. The waves' partial tiles are
 // summed through LDS in a fixed order. What bounds it: one row, the latency of a wave's few units
 // (1 x 4096 x 4096 5.5 us); many words, memory (64 experts' gate and up, 2048 x 7168: 4.2 TB/s);
-// more rows, x's fragments, which every wave loads (37 x 14336 x 4096: 21 us, 1.5 TB/s).
+// more rows, x's fragments, which every wave loads, and for AutoAWQ a unit's words, which nothing
+// runs under (no PRE): 37 x 14336 x 4096 in 21-22 us, 1.5 TB/s, waves waiting 51 % of their cycles.
+// AutoAWQ with PRE or groups of 64: the compiler does not see the waits of the word copies and adds
+// one right behind them, before a unit's scales and x are requested.
 template <int DT, int LAYOUT, int F, int MT, int NT, int SETS, int W>
 struct I4Few {
   static constexpr int T = NT * SETS;
@@ -485,9 +488,10 @@ __global__ __launch_bounds__(64 * W) void k_int4_few(I4Args a) {
 // scaling a tile's products while the next one's run. vLLM: 128 x 32 a wave, words straight to
 // registers, x put into the words' element order on its way to LDS. AutoAWQ: 64 x 64 a wave, words
 // through LDS too (a transposed read gives 64 columns). The sums of x of the next unit's groups are
-// formed one unit ahead, one row tile by each wave. What bounds it: MFMA 44 % and vector
-// instructions 39 % of the issue slots (half of those unpack and scale), at the clock the card
-// keeps under them: 2048 x 14336 x 4096 in 282 us, 850 TF/s, 0.66 of a plain bf16 product's rate.
+// formed one unit ahead, one row tile by each wave. What bounds it: of the time its CU is busy MFMA
+// works 46 % and LDS 38 %, beside 3.0 other vector instructions to a product (half of those unpack
+// and scale); waves wait 33 % of their cycles. 2048 x 14336 x 4096 in 274-290 us, 830-880 TF/s, 0.55
+// of a plain bf16 product's rate of that width.
 constexpr int TM = 128, TX = TM * 256, TW = 128 * 128;  // rows; bytes of an x, a word buffer
 
 template <int LAYOUT>

@@ -102,9 +102,10 @@ struct FwdStage {
 
 // Four waves of 32 query rows share 64-key tiles: scores transposed (a lane holds 32 keys of one
 // row), so that the weights turn into the second product's operand in place. Keys and values stand
-// in two buffers each (80 KB, two workgroups per CU). What bounds it: no unit alone (MFMA 40 %,
-// vector 28 %, LDS 21 % busy) but the chain of phases in a wave, two waves to a SIMD: 2048 tokens
-// of 128 heads in 237 us, 730 TF/s; four padded sequences of 301, 16 heads, 13 us.
+// in two buffers each (80 KB, two workgroups per CU). What bounds it: no unit alone (of the time its
+// CU is busy MFMA works 41 %, LDS 22 %) but the chain of phases in a wave, two waves to a SIMD, which
+// stand at a wait 37 % of their cycles: 2048 tokens of 128 heads in 226-237 us, 725-760 TF/s; four
+// padded sequences of 301, 16 heads, 12-13 us, waiting 53 %.
 // SPLIT: the workgroup takes its share of the query tile's key tiles and leaves the unnormalised
 // output (lane order) with the rows' max and sum for k_mla_fwd_join
 template <int DT, bool SPLIT>
@@ -222,7 +223,9 @@ __global__ void __launch_bounds__(256, 2) k_mla_fwd(MlaFwdArgs a) {
   // Iteration t: the softmax of tile t's scores stands between the products of tile t + 1's (the
   // matrix pipe and the vector pipe work at once), then O^T += V^T P^T. K fragments are read
   // F_AHEAD products ahead (the scheduling barriers keep the compiler to that order: left alone
-  // it waits for each read right before its product)
+  // it waits for each read right before its product). The copies of the tiles after stand behind
+  // the softmax only: the compiler does not see the waits below, holds the queries' loads for
+  // outstanding, and puts a vmcnt(0) of its own before an iteration's first product.
   for (int it = 0; it < ntile; ++it) {
     const int k0 = kbeg + it * FKT;
     const uint32_t cur = lds0 + (it & 1) * F_STAGE, nxt = lds0 + ((it & 1) ^ 1) * F_STAGE;
@@ -500,8 +503,7 @@ __device__ __forceinline__ int dec_len(const MlaDecArgs& a, int b) {
 __device__ __forceinline__ int dec_tiles(const MlaDecArgs& a, int b) {
   return max(1, (dec_len(a, b) + DKT - 1) / DKT);
 }
-// total tiles over all (b, group); with find, also the sequence that holds tile `at` and the first
-// tile of that sequence
+// total tiles over all (b, group)
 __device__ __forceinline__ int dec_total(const MlaDecArgs& a) {
   const int lane = threadIdx.x & 63;
   int n = 0;
@@ -543,8 +545,12 @@ __device__ __forceinline__ int dec_step(const MlaDecArgs& a, int total) {
 // O^T += C^T P^T in place; lane (c, q), register j of output block dt = dim 16 dt + 4 q + j of row
 // c. Element j of a k-step's operands is key 16 (j >> 2) + 4 q + (j & 3).
 // What bounds it: LDS reads, since every wave reads the whole tile for its 16 rows (32 rows a wave
-// would halve that, but queries and outputs would take 512 registers): 32 sequences of up to 8192
-// tokens, 2 x 128 heads, 161 us with the join, 560 TF/s; one sequence of 777, 16 heads, 12 us.
+// would halve that, but queries and outputs would take 512 registers; as it is 21 of the 256 are
+// spilled with 8 waves, 7 with fewer, outside the loop over the tiles): 32 sequences of up to 8192
+// tokens, 2 x 128 heads, 161-172 us with the join, 520-560 TF/s, LDS at work 49 % of the time (a
+// third of it bank conflicts) and MFMA 32 %; one sequence of 777, 16 heads, 12 us. Up to 16 rows
+// (RB 1) the compiler, which does not see the waits below, waits for the queries' loads all through
+// a tile's score products, and so for the copies of the next tile that were just issued.
 template <int DT, int RB, int NST>
 __global__ void __launch_bounds__(64 * RB, 2) k_mla_dec(MlaDecArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char mla_lds[];
@@ -644,7 +650,7 @@ __global__ void __launch_bounds__(64 * RB, 2) k_mla_dec(MlaDecArgs a) {
     for (int tb = t0; tb < t1; tb += dec_tab(NST)) {
     const int te = min(t1, tb + dec_tab(NST));
     p0 = DKT * tb / a.ps;
-    const int np = (min(len, DKT * te) - 1) / a.ps - p0 + 1;  // 0 for an empty sequence
+    const int np = (min(len, DKT * te) - 1) / a.ps - p0 + 1;  // an empty sequence: 0 or 1, unused
     __syncthreads();  // the tiles before are done with the stages and the addresses
     for (int i = tid; i < np; i += 64 * RB) tab[i] = a.table[(int64_t)b * a.nb + p0 + i];
     __syncthreads();
