@@ -329,11 +329,10 @@ def gemm_roofline(kern, elapsed):
 # ---------------------------------------------------------------------------------------
 # CPU baselines (oracle = the reference algorithm on torch-CPU; bounded samples, extrapolated)
 # ---------------------------------------------------------------------------------------
-# auto-clip's VALU issue bound: each SIMD issues one wave64 vector instruction per 2 cycles
-# (MI355X_MICROARCH.md, wave scheduling), and a DT-rounded product costs at least 1/32 of one
-# (v_pk_mul_f32 and v_pk_add_f32 cover 128 products, v_cvt_pk_bf16_f32 64): 1024 SIMDs x
-# 2.4 GHz / 2 x 32 products
-PEAK_CLIP_GPRODUCTS = 1024 * 2.4 / 2 * 32   # 3.93e4 G products/s
+# auto-clip's VALU issue bound: each SIMD issues one wave64 vector instruction per 2 cycles, and
+# 64 DT-rounded products cost at least three (v_mul_f32, v_add_f32, one v_cvt_pk_bf16_f32 per
+# product: the build has no packed fp32 instructions): 1024 SIMDs x 2.4 GHz / 2 x 64 / 3 products
+PEAK_CLIP_GPRODUCTS = 1024 * 2.4 / 2 * 64 / 3   # 2.62e4 G products/s
 
 
 def clip_roofline(kern):
@@ -356,7 +355,8 @@ def clip_roofline(kern):
             'unit': 'G products/s', 'frac': round(gp / PEAK_CLIP_GPRODUCTS, 4),
             'avg_launch_ms': round(ms / launches, 4), 'launches': launches,
             'products_per_launch': flops / launches,
-            'pmc_source': 'profiles/r6_clip_tw_pmc.txt'}
+            'pmc_source': 'profiles/r6_clip_tw_pmc.txt (of a build with packed fp32 '
+                          'multiplies and adds; rates of this one: profiles/clip_rate.txt)'}
 
 
 def cpu_baseline_awq(args, budget_s):
