@@ -741,7 +741,8 @@ int lcq_int4_gemm(const void* x, int dtype, int64_t ldx, int64_t m, int64_t k,
  * [G + 1], ascending; clamped to [0, rows]); rows outside every group are left as they were.
  * With a_rows (DEVICE int64 [rows]) row i reads x row a_rows[i] (out of [0, x_rows): zeros), else
  * x row i. wtab: DEVICE int64 [nsets][G][3] = qweight, scales, qzeros addresses (16-byte aligned
- * but for qzeros, which layout 0 ignores), each [n, k] matrix as above. nsets 2: y [2][rows][n];
+ * but for qzeros, which layout 0 ignores), each [n, k] matrix as above (an address does not say what
+ * it leads to: other weights than these are read out of range). nsets 2: y [2][rows][n];
  * with silu_mul set 0 = gate, set 1 = up and y [rows][n] = rnd(silu(gate) * up), the two products
  * kept in fp32. */
 int lcq_int4_gemm_grouped(const void* x, int dtype, int64_t ldx, int64_t x_rows,
@@ -781,7 +782,8 @@ int lcq_mla_fwd_causal(const void* q_nope, const int64_t* q_nope_strides, const 
  * [B, Sq, H, 512], q_rope [B, Sq, H, 64]: strides {batch, token, head}. kv_lens int32 [B] (clamped
  * to [0, nb * page_size]) counts the Sq new tokens, which are in the cache already. A page number
  * outside [0, pages) hides its tokens; a row without a token is zero; slots past a length are not
- * read. out [B, Sq, H, 512] contiguous. workspace: lcq_mla_decode_workspace_bytes(B, Sq, H, nb *
+ * read. Cached tokens must be finite: with Sq > 1 a NaN or an infinity in a new token can reach the
+ * new tokens before it. out [B, Sq, H, 512] contiguous. workspace: lcq_mla_decode_workspace_bytes(B, Sq, H, nb *
  * page_size) bytes (partial outputs of sequences that several workgroups share; joined in a fixed
  * order: the same call gives the same bits). */
 int64_t lcq_mla_decode_workspace_bytes(int64_t B, int64_t Sq, int64_t H, int64_t max_len);
