@@ -741,8 +741,8 @@ int lcq_int4_gemm(const void* x, int dtype, int64_t ldx, int64_t m, int64_t k,
  * [G + 1], ascending; clamped to [0, rows]); rows outside every group are left as they were.
  * With a_rows (DEVICE int64 [rows]) row i reads x row a_rows[i] (out of [0, x_rows): zeros), else
  * x row i. wtab: DEVICE int64 [nsets][G][3] = qweight, scales, qzeros addresses (16-byte aligned
- * but for qzeros, which layout 0 ignores), each [n, k] matrix as above (an address does not say what
- * it leads to: other weights than these are read out of range). nsets 2: y [2][rows][n];
+ * but for qzeros, which layout 0 ignores), each [n, k] matrix as above (an address does not say
+ * what it leads to: other weights are read out of range). nsets 2: y [2][rows][n];
  * with silu_mul set 0 = gate, set 1 = up and y [rows][n] = rnd(silu(gate) * up), the two products
  * kept in fp32. */
 int lcq_int4_gemm_grouped(const void* x, int dtype, int64_t ldx, int64_t x_rows,

@@ -1660,7 +1660,8 @@ def mla_fwd_causal(q_nope: torch.Tensor, q_rope: torch.Tensor, k_nope: torch.Ten
     projections seen head by head), k_rope [B, Skv, 64] or [B, 1, Skv, 64], one rotary key for all
     heads. Query i stands at position q_start[b] + i (int32 [B]; default Skv - Sq, the queries are
     the last tokens) and sees the keys up to its position below kv_lens[b] (int32 [B]; default
-    Skv); a query that sees none gives zeros. Returns [B, Sq, H, 128] contiguous. Not
+    Skv); a query that sees none gives zeros. Keys below kv_lens must be finite (a NaN there can reach
+    queries that do not see it), those past it are not read. Returns [B, Sq, H, 128] contiguous. Not
     differentiable: an input that requires a gradient is refused."""
     _no_backward('mla_fwd_causal', q_nope, q_rope, k_nope, k_rope, v)
     B, H, Sq, _ = q_nope.shape
@@ -1699,7 +1700,8 @@ def mla_decode(q_latent: torch.Tensor, q_rope: torch.Tensor, ckv: torch.Tensor,
     [B, Sq, H, 64]; ckv [pages, page_size, 512] and k_rope [pages, page_size, 64] (two views of
     one cache, or two caches; any strides with a contiguous last dim); block_table int32 [B, nb]
     names the pages of each sequence, kv_lens int32 [B] its tokens, the Sq new ones included: new
-    token i sees the first kv_lens - Sq + i + 1. A page number outside the cache hides its tokens;
+    token i sees the first kv_lens - Sq + i + 1 (cached tokens must be finite: a NaN in a new token
+    can reach those before it). A page number outside the cache hides its tokens;
     a row that sees none gives zeros. Returns the attended latents [B, Sq, H, 512] contiguous. Not
     differentiable: an input that requires a gradient is refused."""
     _no_backward('mla_decode', q_latent, q_rope, ckv, k_rope)
