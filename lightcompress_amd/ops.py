@@ -1504,17 +1504,25 @@ def int4_linear(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor,
 
 class Int4Table(torch.Tensor):
     """Addresses of packed weights, and in ``int4`` what they lead to: (layout, n, k, group). What
-    torch makes of tables (stack, slices, copies) is a table of the same weights, of none where
-    they differ (``int4`` None)."""
+    torch puts together of tables (stack, cat, slices, copies) is a table of the same weights, of
+    none where they differ (``int4`` None); anything else, written or computed, is none."""
 
     int4 = None
+    _KEEP = frozenset(('stack', 'cat', 'clone', 'contiguous', 'to', 'cuda', 'cpu', 'detach',
+                       '__getitem__', 'copy_'))
 
     @classmethod
     def __torch_function__(cls, func, types, args=(), kwargs=None):
         out = super().__torch_function__(func, types, args, kwargs or {})
+        name = getattr(func, '__name__', '')
+        if name == '__setitem__':
+            args[0].int4 = None
         if isinstance(out, Int4Table):
-            flat = [u for t in args for u in (t if isinstance(t, (list, tuple)) else (t,))]
-            kinds = {t.int4 for t in flat if isinstance(t, Int4Table)}
+            kinds = {None}
+            if name in cls._KEEP:
+                src = args[1:2] if name == 'copy_' else args[:1]   # copy_ leaves nothing of its own
+                src = src[0] if src and isinstance(src[0], (list, tuple)) else src
+                kinds = {getattr(t, 'int4', None) for t in src}
             out.int4 = kinds.pop() if len(kinds) == 1 else None
         return out
 

@@ -50,8 +50,8 @@ def test_tables_of_different_weights_do_not_mix():
     with pytest.raises(ValueError, match='int4_weight_table'):
         product(torch.stack([a, b]))
     c = ops.int4_weight_table(weights('vllm'), 'cpu')
-    c.copy_(b)
-    with pytest.raises(ValueError, match='int4_weight_table'):
+    c.copy_(b)                                                 # now a table of b's weights
+    with pytest.raises(ValueError, match='wtab holds'):
         product(c)
 
 
@@ -66,6 +66,20 @@ def test_a_table_stays_one_where_tensors_do():
     off = torch.zeros(G, dtype=torch.int64)                    # as many groups as row_off names
     with pytest.raises(ValueError, match='row_off'):
         ops.int4_linear_grouped(torch.zeros(5, K, dtype=torch.bfloat16), off, tab, NC, 128)
+
+
+def test_what_is_computed_from_a_table_is_none():
+    """New contents, a memory of the same shape, arithmetic: no addresses of those weights."""
+    tab = ops.int4_weight_table(weights('vllm'), 'cpu')
+    written, added = tab.clone(), tab.clone()
+    written[0] = torch.zeros(3, dtype=torch.int64)
+    added.add_(16)
+    for t in (torch.empty_like(tab), torch.zeros_like(tab), tab + 16, tab.flip(0), written, added,
+              tab.clone().zero_(), tab.clone().copy_(torch.zeros(G, 3, dtype=torch.int64))):
+        with pytest.raises(ValueError, match='int4_weight_table'):
+            product(t)
+    with pytest.raises(N.LcqError, match='GPU only'):
+        product(tab)
 
 
 class Elsewhere(torch.Tensor):
