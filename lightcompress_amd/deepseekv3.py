@@ -12,6 +12,7 @@ and deploy. Block-fp8 checkpoints (``torch_dtype: torch.float8_e4m3fn``,
 """
 from __future__ import annotations
 
+import itertools
 import types
 
 import torch
@@ -303,7 +304,7 @@ def _lcq_mla_past(attn, x, position_embeddings, attention_mask, past_key_values,
             or attention_mask is not None or kwargs.get('output_attentions')
             or kwargs.get('is_causal') is False
             or (attn.training and attn.attention_dropout)
-            or _needs_grad([x, *position_embeddings, *attn.parameters()])
+            or _needs_grad(itertools.chain([x], position_embeddings, attn.parameters()))
             or attn.config._attn_implementation != 'sdpa'
             or (attn.qk_nope_head_dim, attn.qk_rope_head_dim, attn.v_head_dim,
                 attn.kv_lora_rank) != (128, 64, 128, 512)):
@@ -349,8 +350,9 @@ def _lcq_mla_forward(self, hidden_states, position_embeddings, attention_mask,
     q_rot, k_rot = rope(q_rot, k_rot, cos, sin)
     if past_key_values is not None:
         ckv, k_rot = past_key_values.update(ckv, k_rot, self.layer_idx)
-        # a preallocated cache gives its whole buffer: the tokens so far are its first ones
-        ckv, k_rot = ckv[:, :, :past + S], k_rot[:, :, :past + S]
+        if ckv.shape[2] > past + S:
+            # a preallocated cache gives its whole buffer: the tokens so far are its first ones
+            ckv, k_rot = ckv[:, :, :past + S], k_rot[:, :, :past + S]
     T = ckv.shape[2]
     w = _plain_weight(self.kv_b_proj) if past else None
     if w is not None and w.dtype == q.dtype:
