@@ -177,7 +177,7 @@ class ExpertList(nn.ModuleList):
         rebuilt when any of them changed (the modules keep the tensors). A table that is replaced
         is not reused for other memory before the streams that read it are done with it, and never
         one that a graph was captured with."""
-        from . import ops
+        from . import _native as N, ops
         from .module_utils import int4_weight
         ws = [[int4_weight(getattr(mlp, p)) for mlp in self]
               for p in ('gate_proj', 'up_proj', 'down_proj')]
@@ -190,12 +190,15 @@ class ExpertList(nn.ModuleList):
                                    'addresses and cannot be captured; run the step once before')
             gate, up, down = ws
             cached = (key, (ops.int4_weight_table(gate, device, up),
-                            ops.int4_weight_table(down, device)))
+                            ops.int4_weight_table(down, device)), set())
             self._lcq_int4_tables = cached
-        tables = cached[1]
+        _, tables, streams = cached
         if device.type == 'cuda':
-            for t in tables:
-                t.record_stream(torch.cuda.current_stream(device))
+            stream = N.stream_of(tables[0])
+            if stream not in streams:             # once: what it has queued by then is waited for
+                streams.add(stream)
+                for t in tables:
+                    t.record_stream(torch.cuda.current_stream(device))
             if _capturing():
                 kept = self.__dict__.setdefault('_lcq_int4_captured', [])
                 if not any(t is tables for t in kept):
