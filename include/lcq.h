@@ -783,9 +783,9 @@ int lcq_mla_fwd_causal(const void* q_nope, const int64_t* q_nope_strides, const 
  * to [0, nb * page_size]) counts the Sq new tokens, which are in the cache already. A page number
  * outside [0, pages) hides its tokens; a row without a token is zero; slots past a length are not
  * read. Cached tokens must be finite: with Sq > 1 a NaN or an infinity in a new token can reach the
- * new tokens before it. out [B, Sq, H, 512] contiguous. workspace: lcq_mla_decode_workspace_bytes(B, Sq, H, nb *
- * page_size) bytes (partial outputs of sequences that several workgroups share; joined in a fixed
- * order: the same call gives the same bits). */
+ * new tokens before it. out [B, Sq, H, 512] contiguous. workspace:
+ * lcq_mla_decode_workspace_bytes(B, Sq, H, nb * page_size) bytes (partial outputs of sequences that
+ * several workgroups share; joined in a fixed order: the same call gives the same bits). */
 int64_t lcq_mla_decode_workspace_bytes(int64_t B, int64_t Sq, int64_t H, int64_t max_len);
 int lcq_mla_decode(const void* q_latent, const int64_t* q_latent_strides, const void* q_rope,
                    const int64_t* q_rope_strides, const void* ckv, const int64_t* ckv_strides,
